@@ -138,6 +138,67 @@ int rvm_metrics_static(const float* pred_pha, const float* true_pha, const float
                        const float* pred_fgr, const float* true_fgr, int N, int H, int W, double sigma,
                        double* sums, void* hip_stream);
 
+/* ---- Temporal operators (no counterpart in the reference, whose only memory of a stream is the ConvGRU state) ------------
+ * The two other ways of carrying a stream's past, under rvm_forward's contract: the caller owns the state, and one call
+ * with T steps gives what T calls with one step give.
+ *   rvm_causal_conv, rvm_selective_scan : a state of fixed size (the last W-1 inputs; N states per channel)
+ *   rvm_append_kv, rvm_attend           : a paged key-value cache of the stream's tokens and the attention that reads it
+ * dtype names the tensors' type as in rvm_compose_u8 (fp32; fp16; bf16); sums, states and softmax statistics are fp32.
+ * Strides are in elements; the channel / head dimension is dense.  Work is enqueued on `hip_stream` on the calling thread's
+ * CURRENT device, which must own the buffers; no allocation, no synchronisation (capturable).  Inference only: no gradients.
+ * Structs are zero-initialised by callers that leave optional fields out. */
+
+/* y[b,t,d] = act(bias[d] + sum_w weight[w,d] * xx[b,t+w,d]), xx = the W-1 rows of state_in (NULL: zeros) followed by x;
+ * act = silu or none.  state_out receives the last W-1 rows of xx; it must not overlap state_in, x or y. */
+typedef struct rvm_conv_args {
+    const void *x, *weight, *bias, *state_in;   /* [B,T,D] by strides, [W,D], [D] or NULL, [B,W-1,D] or NULL */
+    void *y, *state_out;                        /* [B,T,D], [B,W-1,D] dense */
+    int64_t x_sb, x_st, B, T, D, W, silu;       /* W = 2..4 */
+} rvm_conv_args;
+int rvm_causal_conv(int dtype, const rvm_conv_args* args, void* hip_stream);
+
+/* delta = softplus(dt + dt_bias) (or dt + dt_bias with softplus = 0);  h_t = exp(delta_t * A) * h_(t-1) + delta_t * x_t * B_t;
+ * y_t = sum_n C_t[n] h_t[n] + D * x_t, times z_t * sigmoid(z_t) where z is given.  State h [B,N,D] in fp32; state_out may be
+ * state_in.  Workspace: rvm_selective_scan_workspace bytes (0: none), free for reuse when the call's work is done. */
+typedef struct rvm_scan_args {
+    const void *x, *dt, *z, *B, *C;             /* [B,T,D] x 3 (z may be NULL), [B,T,N] x 2, by strides */
+    const float *A, *D, *dt_bias, *state_in;    /* [N,D]; [D], [D], [B,N,D] or NULL */
+    void* y; float* state_out; void* workspace; /* [B,T,D], [B,N,D] dense */
+    int64_t x_sb, x_st, dt_sb, dt_st, z_sb, z_st, B_sb, B_st, C_sb, C_st;
+    int64_t nB, nT, nD, nN, softplus, workspace_bytes;      /* nN = 1..64 */
+} rvm_scan_args;
+int64_t rvm_selective_scan_workspace(int64_t B, int64_t T, int64_t D, int64_t N);
+int rvm_selective_scan(int dtype, const rvm_scan_args* args, void* hip_stream);
+
+/* Paged cache: pools k_pages, v_pages [pages][Hkv][page][Dh]; position p of stream s lives in page table[s][p / page], slot
+ * p % page.  New tokens are packed rows: offsets [S+1] gives every stream's rows (NULL: one row per stream, M == S), and its
+ * i-th row has position lengths[s] + i (lengths: tokens BEFORE this call, for append and attend alike).  All three are
+ * device int32, so a captured call follows the cache as it grows.  A negative position is no token: nothing is stored, its
+ * attention is 0.  Rows behind the last stream's come out as 0.  A page number outside the pool, or a column past the table,
+ * is never followed: append drops the token, and attention over it is NaN.
+ * page: a power of two, 16..1024.  Dh: a multiple of 8 up to 256.
+ *
+ * rvm_append_kv stores k and v [M,Hkv,Dh]; the first `rot` dims of k, and of q [M,Hq,Dh] into q_out where given, are rotated
+ * by position * freqs[i] (angle in 64 bits): pairs (i, i + rot/2), or (2i, 2i+1) with `interleaved`. */
+typedef struct rvm_append_args {
+    const void *q, *k, *v; void *q_out, *k_pages, *v_pages;     /* q, q_out may be NULL (both) */
+    const int32_t *table, *lengths, *offsets; const float* freqs;
+    int64_t q_sm, q_sh, k_sm, k_sh, v_sm, v_sh;                 /* row and head strides */
+    int64_t M, S, Hq, Hkv, Dh, pages, page, width, rot, interleaved;    /* width: columns of the table; rot: multiple of 16 */
+} rvm_append_args;
+int rvm_append_kv(int dtype, const rvm_append_args* args, void* hip_stream);
+
+/* out[m,h] = sum_j softmax_j(scale * q[m,h] . k_j) v_j over the positions j <= the row's own; query head h reads key head
+ * h / (Hq / Hkv).  Append the rows' own keys first. */
+typedef struct rvm_attend_args {
+    const void *q, *k_pages, *v_pages; void *out, *workspace;   /* [M,Hq,Dh] by strides; out dense */
+    const int32_t *table, *lengths, *offsets;
+    int64_t q_sm, q_sh, M, S, Hq, Hkv, Dh, pages, page, width, workspace_bytes;
+    double scale;
+} rvm_attend_args;
+int64_t rvm_attend_workspace(int dtype, const rvm_attend_args* args);   /* by sizes alone; -1: refused */
+int rvm_attend(int dtype, const rvm_attend_args* args, void* hip_stream);
+
 /* Debug / test taps: copy an intermediate activation of the LAST forward to host as fp32 NCHW.
  * Names: s0 s1 s2 s3 f1 f2 f3 f4 aspp x3 x2 x1 hid ab.  Synchronises the device. */
 int rvm_debug_tap(rvm_ctx* ctx, const char* name, float* host_out, int64_t capacity, int64_t shape[4]);

@@ -1829,6 +1829,8 @@ int plan_impl(rvm_ctx* c, int B, int T, int H, int W, double ds) {
 // =============================================================================================
 // C ABI
 // =============================================================================================
+int rvm_set_error(const std::string& m) { return fail(m); }        // for the entry points of the other files
+
 extern "C" {
 
 const char* rvm_last_error(void) { return g_err.c_str(); }

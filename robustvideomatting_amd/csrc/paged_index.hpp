@@ -1,0 +1,16 @@
+// Where a position of a stream lives in a paged cache.  Plain C++ on both sides, so that the bounds can be checked on the host.
+#pragma once
+#include <stdint.h>
+#ifdef __HIPCC__
+#define RVM_HD __host__ __device__ __forceinline__
+#else
+#define RVM_HD inline
+#endif
+// Page of position `pos` (>= 0) of stream s, or -1 where the table has none: a column past its end, a page number outside
+// the pool.  The table is read in bounds whatever the caller's lengths hold.
+RVM_HD int page_of(const int* table, int width, int pages, int page_shift, int s, int pos) {
+    const int col = pos >> page_shift;
+    if (pos < 0 || col >= width) return -1;
+    const int pg = table[(int64_t)s * width + col];
+    return (unsigned)pg < (unsigned)pages ? pg : -1;
+}

@@ -19,7 +19,8 @@ REFINERS = {"deep_guided_filter": 0, "fast_guided_filter": 1}
 SYMBOLS = [
     "rvm_create", "rvm_destroy", "rvm_param_count", "rvm_param_name", "rvm_param_shape",
     "rvm_set_param", "rvm_finalize", "rvm_plan", "rvm_plan_seq", "rvm_memory_bytes", "rvm_trim", "rvm_state_shape", "rvm_forward", "rvm_forward_u8",
-    "rvm_debug_tap", "rvm_debug_stamps", "rvm_compose_u8", "rvm_metrics", "rvm_metrics_workspace", "rvm_metrics_static", "rvm_metrics_static_capacity", "rvm_launch_count", "rvm_launch_kernels", "rvm_launch_info", "rvm_profile_frame", "rvm_set_graph_mode", "rvm_set_frame_pipeline", "rvm_frame_pipeline_src_event", "rvm_last_error", "rvm_version",
+    "rvm_debug_tap", "rvm_debug_stamps", "rvm_compose_u8", "rvm_metrics", "rvm_metrics_workspace", "rvm_metrics_static", "rvm_metrics_static_capacity", "rvm_launch_count", "rvm_launch_kernels", "rvm_launch_info", "rvm_profile_frame", "rvm_set_graph_mode", "rvm_set_frame_pipeline", "rvm_frame_pipeline_src_event",
+    "rvm_causal_conv", "rvm_selective_scan", "rvm_selective_scan_workspace", "rvm_append_kv", "rvm_attend", "rvm_attend_workspace", "rvm_last_error", "rvm_version",
 ]
 
 _lib = None
@@ -100,6 +101,19 @@ def lib():
     L.rvm_set_frame_pipeline.restype = ci
     L.rvm_frame_pipeline_src_event.argtypes = [vp, vp]
     L.rvm_frame_pipeline_src_event.restype = ci
+    i64, args = ctypes.c_int64, ctypes.c_char_p         # argument blocks are packed bytes (temporal.py)
+    L.rvm_causal_conv.argtypes = [ci, args, vp]
+    L.rvm_causal_conv.restype = ci
+    L.rvm_selective_scan_workspace.argtypes = [i64, i64, i64, i64]
+    L.rvm_selective_scan_workspace.restype = i64
+    L.rvm_selective_scan.argtypes = [ci, args, vp]
+    L.rvm_selective_scan.restype = ci
+    L.rvm_append_kv.argtypes = [ci, args, vp]
+    L.rvm_append_kv.restype = ci
+    L.rvm_attend_workspace.argtypes = [ci, args]
+    L.rvm_attend_workspace.restype = i64
+    L.rvm_attend.argtypes = [ci, args, vp]
+    L.rvm_attend.restype = ci
     L.rvm_last_error.argtypes = []
     L.rvm_last_error.restype = ctypes.c_char_p
     L.rvm_version.argtypes = []
