@@ -1,69 +1,676 @@
-// Attention of new tokens over a paged key-value cache.
+// Attention of new tokens over a paged key-value cache: softmax_j(scale q . k_j) v_j, one pass over the cache with a running
+// maximum and sum.  Both kernels compute the transposed products
+//     S' = K Q'   (keys x rows)        O' = V' P'   (dims x rows)
+// because the accumulator of the first then holds, per lane, scores of ONE row: its maximum and sum are in-lane but for one or
+// two exchanges, the rescale of O' is a lane's own, and the weights P' are the B operand of the second product where they
+// stand - the matrix instruction sums over its K slots in any order, so V' is simply read in the order the scores came out.
+//   attend_one    one new token per stream: the rows of a tile are the query heads that share a key head (16 x 16 tiles)
+//   attend_chunk  many rows per stream: (token, head of the group) pairs share every key they read (32 x 32 tiles)
 #include "temporal.hpp"
 
 namespace {
 
-// One wave per (row, query head), 64 keys at a time: a lane scores one key, then every lane sums its dims over the 64.
-template <typename T>
-__global__ __launch_bounds__(64) void attend_rows(AttendArgs a) {
-    __shared__ float qs[256];
-    __shared__ float ps[64];
-    const int m = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef Vec<bfl, 8>::type b16x8;
+
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// ---- a tile of keys or values in LDS: rows of DP elements in 16-byte pieces, the pieces of a row permuted by XOR so that the
+// reads below spread over all banks (64 banks of 4 bytes: 16 pieces side by side; RPL rows of a narrow tile share a line)
+template <typename T, int DP> struct Tile {
+    static constexpr int PER = 16 / (int)sizeof(T), CPR = DP / PER, RPL = CPR >= 16 ? 1 : 16 / CPR, PITCH = DP * (int)sizeof(T);
+    // keys: 16 rows, the same piece of each
+    __device__ static __forceinline__ int kswz(int row, int c) { return c ^ ((row / RPL) & (CPR < 16 ? CPR - 1 : 15)); }
+    // values, 16-bit: 8 rows, the same two pieces of each (transposing read); fp32: rows 4 apart, the same four (or eight)
+    __device__ static __forceinline__ int vswz(int row, int c) {
+        if constexpr (sizeof(T) == 2) return c ^ (((row / RPL) << 1) & (CPR < 16 ? CPR - 1 : 15));
+        else return c ^ ((((row >> 2) & 3) << 2) & (CPR - 1));
+    }
+    __device__ static __forceinline__ int koff(int row, int c) { return row * PITCH + kswz(row, c) * 16; }
+    __device__ static __forceinline__ int voff(int row, int c) { return row * PITCH + vswz(row, c) * 16; }
+};
+// four rows x 16 columns of 16-bit elements, transposed: lane i of 16 gets column i of rows 0..3; the address of lane i is
+// that of row i / 4, columns 4 (i % 4) ..
+__device__ __forceinline__ s16x4 read_tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(b16x8 a, b16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(b16x8 a, b16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+
+template <typename V> __device__ __forceinline__ V as(u32x4 v) { return __builtin_bit_cast(V, v); }
+template <typename T> __device__ __forceinline__ u32x4 piece(const T* p, bool ok) {
+    u32x4 z = {0, 0, 0, 0};
+    if (ok) z = *(const u32x4*)p;
+    return z;
+}
+
+// ---- one token per stream -------------------------------------------------------------------------------------------------
+// Work is cut by keys, not by streams: all streams' caches in units of NW tiles laid end to end, and block b of the grid
+// takes the b-th equal share, whatever the streams' lengths - they are known on the device only.  A (stream, key head, 16 query
+// heads) segment that fits inside a share is finished there; the pieces of one that does not go to the workspace (a block
+// has at most two such pieces: its first and its last) and attend_join adds them up in order.
+template <typename T> constexpr int one_kt() { return sizeof(T) == 2 ? 32 : 16; }         // keys per tile of a wave
+template <int DP> constexpr int one_nw() { return DP > 128 ? 2 : 4; }                      // waves of a block
+constexpr int ONE_ROWS = 16, ONE_GRID = 512;
+constexpr int piece_floats(int DP) { return ONE_ROWS * (DP + 2); }
+
+// Where unit u of all units lies.  Run by a whole wave; uniform results.
+struct Units {
+    int64_t total, per;                 // units in all, of a block's share
+    int stream, units;                  // stream of the unit asked for, units of each of its segments
+    int64_t first;                      // first unit of that stream
+    __device__ __forceinline__ static int of_stream(const PagedArgs& p, int s, int keys) {
+        const int pos = s < p.S ? p.lengths[s] : -1;
+        return pos < 0 ? 0 : pos / keys + 1;
+    }
+    __device__ __forceinline__ void sum(const PagedArgs& p, int keys, int segs) {
+        int64_t t = 0;
+        for (int b = 0; b < p.S; b += 64) t += of_stream(p, b + (threadIdx.x & 63), keys);
+        for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
+        total = t * segs;
+        per = (total + ONE_GRID - 1) / ONE_GRID;
+    }
+    // sets stream, units, first for unit u (0 <= u < total)
+    __device__ __forceinline__ void find(const PagedArgs& p, int keys, int segs, int64_t u) {
+        int64_t before = 0;
+        const int lane = threadIdx.x & 63;
+        for (int b = 0; b < p.S; b += 64) {
+            const int mine = of_stream(p, b + lane, keys);
+            int64_t inc = (int64_t)mine * segs;
+            for (int o = 1; o < 64; o <<= 1) { const int64_t v = __shfl_up(inc, o); if (lane >= o) inc += v; }
+            const unsigned long long hit = __ballot(before + inc > u);
+            if (hit) {
+                const int l = __ffsll(hit) - 1;
+                stream = b + l;
+                units = __shfl(mine, l);
+                first = before + __shfl(inc, l) - (int64_t)units * segs;
+                return;
+            }
+            before += __shfl(inc, 63);
+        }
+        stream = -1; units = 1; first = 0;
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_one(AttendArgs a) {
+    constexpr int NW = one_nw<DP>(), KT = one_kt<T>(), KEYS = NW * KT;
+    typedef Tile<T, DP> TL;
+    constexpr int LD = KT * TL::CPR / 64;                       // 16-byte pieces per lane of a K (or V) tile
+    constexpr int DT = DP / 16, TILE_BYTES = KT * TL::PITCH;
+    __shared__ __attribute__((aligned(16))) char lds[NW * 2 * TILE_BYTES];
+    __shared__ float red_m[NW][16], red_l[NW][16];
     const PagedArgs& p = a.p;
-    const int Dh = p.Dh, kvh = h / (p.Hq / p.Hkv);
-    int pos;
-    const int s = __builtin_amdgcn_readfirstlane(paged_row(p, m, pos));
-    T* out = (T*)a.out + ((int64_t)m * p.Hq + h) * Dh;
-    if (s >= p.S || pos < 0) {
-        for (int d = lane; d < Dh; d += 64) out[d] = (T)0.f;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int group = p.Hq / p.Hkv, rts = (group + 15) / 16, segs = p.Hkv * rts, Dh = p.Dh;
+    char* kt_lds = lds + wave * 2 * TILE_BYTES;
+    char* vt_lds = kt_lds + TILE_BYTES;
+
+    Units U;
+    U.sum(p, KEYS, segs);
+    int64_t u0, u1;
+    if (a.splits) { u0 = blockIdx.x * U.per; u1 = min(U.total, u0 + U.per); }
+    else {                                                      // a block per segment, no pieces
+        const int s = blockIdx.x / segs;
+        int64_t before = 0;
+        for (int b = 0; b < s; b += 64) before += b + lane < s ? Units::of_stream(p, b + lane, KEYS) : 0;
+        for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
+        const int n = Units::of_stream(p, s, KEYS);
+        u0 = before * segs + (int64_t)(blockIdx.x % segs) * n; u1 = u0 + n;
+    }
+    // a stream without tokens (and its rows) has no unit: its rows are 0
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + tid; i < (int64_t)p.S * p.Hq; i += (int64_t)gridDim.x * blockDim.x) {
+        const int s = (int)(i / p.Hq);
+        if (p.lengths[s] < 0)
+            for (int d = 0; d < Dh; d += 8)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ((T*)a.out)[i * Dh + d + k] = (T)0.f;
+    }
+    while (u0 < u1) {
+        U.find(p, KEYS, segs, u0);
+        const int s = __builtin_amdgcn_readfirstlane(U.stream), n_units = __builtin_amdgcn_readfirstlane(U.units);
+        const int seg = (int)((u0 - U.first) / n_units);
+        const int64_t seg0 = U.first + (int64_t)seg * n_units;
+        const int ua = (int)(u0 - seg0), ub = (int)min((int64_t)n_units, u1 - seg0);        // units of the segment done here
+        const int kvh = seg / rts, h0 = kvh * group + (seg - kvh * rts) * 16, rows = min(16, kvh * group + group - h0);
+        const int pos = p.lengths[s];
+        const int t_end = ub * NW;                              // tiles, interleaved over the waves
+        // ---- Q fragments: lane l15 is the row
+        f32x4 acc[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+        u32x4 qf[TL::CPR / 4];
+        const T* q = (const T*)a.q + s * a.q_sm + (h0 + min(l15, rows - 1)) * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 4; ++i) qf[i] = piece(q + (4 * i + g) * TL::PER, (4 * i + g) * TL::PER < Dh);
+        float m = -INFINITY, l = 0.f;
+        bool lost = false;
+        u32x4 kr[LD], vr[LD];
+        int pg[2];
+        auto pages = [&](int t) {
+            const int k0 = t * KT;
+            pg[0] = k0 <= pos ? paged_page(p, s, k0) : -2;
+            if (KT > 16) pg[1] = k0 + 16 <= pos ? paged_page(p, s, k0 + 16) : -2;
+            lost |= pg[0] == -1 || (KT > 16 && pg[1] == -1);
+        };
+        auto load = [&](int t) {
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                const int i = j * 64 + lane, row = i / TL::CPR, pc = i % TL::CPR, key = t * KT + row;
+                const int page = KT > 16 && row >= 16 ? pg[1] : pg[0];
+                const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * Dh;
+                const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
+                const bool ok = page >= 0 && key <= pos;
+                kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
+                vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
+            }
+        };
+        int t = ua * NW + wave;
+        if (t < t_end) { pages(t); load(t); if (t + NW < t_end) pages(t + NW); }
+        for (; t < t_end; t += NW) {
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                *(u32x4*)(kt_lds + (j * 64 + lane) * 16) = kr[j];
+                *(u32x4*)(vt_lds + (j * 64 + lane) * 16) = vr[j];
+            }
+            if (t + NW < t_end) { load(t + NW); if (t + 2 * NW < t_end) pages(t + 2 * NW); }
+            // ---- scores: lane = (row l15, keys 4 g .. 4 g + 3 of each 16)
+            f32x4 sc[KT / 16];
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; ++kt) {
+                sc[kt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < TL::CPR / 4; ++i) {
+                    const u32x4 kf = *(const u32x4*)(kt_lds + TL::koff(kt * 16 + l15, 4 * i + g));
+                    if constexpr (sizeof(T) == 2) sc[kt] = mma16(as<typename Vec<T, 8>::type>(kf), as<typename Vec<T, 8>::type>(qf[i]), sc[kt]);
+                    else
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) sc[kt] = mma16(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
+                }
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; ++kt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float v = sc[kt][c] * a.scale_log2e;
+                    sc[kt][c] = t * KT + kt * 16 + 4 * g + c <= pos ? v : -INFINITY;
+                    mt = fmaxf(mt, sc[kt][c]);
+                }
+            mt = fmaxf(mt, __shfl_xor(mt, 16));
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn, al = exp2_hw(m - ms);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] *= al;
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; ++kt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { sc[kt][c] = exp2_hw(sc[kt][c] - ms); l += sc[kt][c]; }
+            if constexpr (sizeof(T) == 2) {
+                typename Vec<T, 8>::type pf;                    // weights rounded to the tensors' type for the matrix instruction
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { pf[c] = (T)sc[0][c]; pf[4 + c] = (T)sc[1][c]; }
+#pragma unroll
+                for (int i = 0; i < DT; ++i) {
+                    const int r = 4 * g + (l15 >> 2), c = 2 * i + ((l15 >> 1) & 1), o = (l15 & 1) * 8;
+                    s16x4 v[2] = {read_tr(vt_lds + TL::voff(r, c) + o), read_tr(vt_lds + TL::voff(r + 16, c) + o)};
+                    acc[i] = mma16(__builtin_bit_cast(typename Vec<T, 8>::type, v), pf, acc[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float v = *(const float*)(vt_lds + TL::voff(4 * g + c, 4 * i + (l15 >> 2)) + (l15 & 3) * 4);
+                        acc[i] = mma16(v, sc[0][c], acc[i]);
+                    }
+            }
+        }
+        // ---- the waves' parts joined: maxima and sums first, then each wave adds its scaled part
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (__any(lost)) l = NAN;
+        __syncthreads();                                        // the tiles are free
+        if (g == 0) { red_m[wave][l15] = m; red_l[wave][l15] = l; }
+        float* sum = (float*)lds;                               // [16 rows][DP + 4]
+        constexpr int SP = DP + 4;
+        __syncthreads();
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, red_m[w][l15]);
+        const float MS = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) L += red_l[w][l15] * exp2_hw(red_m[w][l15] - MS);
+        const float mine = exp2_hw(m - MS);
+        for (int w = 0; w < NW; ++w) {
+            if (wave == w)
+#pragma unroll
+                for (int i = 0; i < DT; ++i) {
+                    f32x4* d = (f32x4*)(sum + l15 * SP + i * 16 + g * 4);
+                    *d = w ? *d + acc[i] * mine : acc[i] * mine;
+                }
+            __syncthreads();
+        }
+        const bool whole = ua == 0 && ub == n_units;
+        if (tid < 16) { red_m[0][tid] = M; red_l[0][tid] = L; }     // (each lane of the first 16 holds its own row's)
+        __syncthreads();
+        if (whole) {
+            for (int i = tid; i < rows * Dh; i += 64 * NW) {
+                const int r = i / Dh, d = i - r * Dh;
+                ((T*)a.out)[((int64_t)s * p.Hq + h0 + r) * Dh + d] = (T)(sum[r * SP + d] / red_l[0][r]);
+            }
+        } else {
+            float* o = a.part + ((int64_t)blockIdx.x * 2 + (ua == 0)) * piece_floats(DP);       // slot 0: began in an earlier share
+            for (int i = tid; i < rows * DP; i += 64 * NW) o[i] = sum[(i / DP) * SP + i % DP];
+            if (tid < rows) { o[ONE_ROWS * DP + tid] = red_m[0][tid]; o[ONE_ROWS * (DP + 1) + tid] = red_l[0][tid]; }
+        }
+        __syncthreads();
+        u0 = seg0 + ub;
+    }
+}
+
+// Adds the pieces of the segments that no block of attend_one had whole, in the order of the keys.  One block per segment.
+template <typename T, int DP>
+__global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
+    const PagedArgs& p = a.p;
+    const int group = p.Hq / p.Hkv, rts = (group + 15) / 16, segs = p.Hkv * rts, lane = threadIdx.x & 63;
+    const int s = blockIdx.x / segs, seg = blockIdx.x % segs, d = threadIdx.x;
+    const int n = Units::of_stream(p, s, keys);
+    if (!n) return;
+    Units U;
+    U.sum(p, keys, segs);
+    int64_t before = 0;
+    for (int b = 0; b < s; b += 64) before += b + lane < s ? Units::of_stream(p, b + lane, keys) : 0;
+    for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
+    const int64_t first = before * segs + (int64_t)seg * n, b0 = first / U.per, b1 = (first + n - 1) / U.per;
+    if (b0 == b1) return;
+    const int kvh = seg / rts, h0 = kvh * group + (seg - kvh * rts) * 16, rows = min(16, kvh * group + group - h0);
+    for (int r = 0; r < rows; ++r) {
+        float M = -INFINITY, L = 0.f, acc = 0.f;
+        for (int64_t b = b0; b <= b1; ++b) {
+            const float* o = a.part + (b * 2 + (b == b0)) * piece_floats(DP);
+            const float m = o[ONE_ROWS * DP + r], l = o[ONE_ROWS * (DP + 1) + r], mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
+            const float ea = exp2_hw(M - ms), eb = exp2_hw(m - ms);
+            acc = acc * ea + o[r * DP + d] * eb;
+            L = L * ea + l * eb;
+            M = mn;
+        }
+        if (d < p.Dh) ((T*)a.out)[((int64_t)s * p.Hq + h0 + r) * p.Dh + d] = (T)(acc / L);
+    }
+}
+
+// ---- many rows per stream -------------------------------------------------------------------------------------------------
+template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
+constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_chunk(AttendArgs a) {
+    constexpr int KT = chunk_kt<T>(), NK = KT / 32, R = 32 * NW, NT = 64 * NW, DT = DP / 32;
+    typedef Tile<T, DP> TL;
+    constexpr int LD = KT * TL::CPR / NT, TILE_BYTES = KT * TL::PITCH;
+    typedef typename Vec<T, 8>::type V8;
+    extern __shared__ __attribute__((aligned(16))) char lds[];              // two buffers of a K and a V tile, flags
+    unsigned long long* flag = (unsigned long long*)(lds + 4 * TILE_BYTES); // [2]: rows of a V tile that are not finite
+    const PagedArgs& p = a.p;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, hf = lane >> 5;
+    const int group = p.Hq / p.Hkv, Dh = p.Dh;
+    const int kvh = blockIdx.x % p.Hkv, tile_id = blockIdx.x / p.Hkv;
+    // ---- rows of no stream are 0
+    if (kvh == 0 && blockIdx.y == 0) {
+        const int lo = min(max(p.offsets[0], 0), p.M), hi = min(max(p.offsets[p.S], 0), p.M), none = lo + p.M - hi;
+        for (int r = tile_id; r < none; r += gridDim.x / p.Hkv) {
+            T* o = (T*)a.out + (int64_t)(r < lo ? r : hi + r - lo) * p.Hq * Dh;
+            for (int i = tid; i < p.Hq * Dh; i += NT) o[i] = (T)0.f;
+        }
+    }
+    // ---- stream and rows of this block: the streams' row tiles laid end to end, a stream's last (longest) tile first
+    int s = -1, row0 = 0, n_rows = 0, start = 0;
+    {
+        int64_t before = 0;
+        for (int b = 0; b < p.S && s < 0; b += 64) {
+            int lo = 0, n = 0;
+            if (b + lane < p.S) {
+                lo = min(max(p.offsets[b + lane], 0), p.M);
+                n = max(0, min(p.offsets[b + lane + 1], p.M) - lo);
+            }
+            const int64_t mine = ((int64_t)n * group + R - 1) / R;
+            int64_t inc = mine;
+            for (int o = 1; o < 64; o <<= 1) { const int64_t v = __shfl_up(inc, o); if (lane >= o) inc += v; }
+            const unsigned long long hit = __ballot(before + inc > tile_id);
+            if (hit) {
+                const int l = __ffsll(hit) - 1;
+                const int64_t end = before + __shfl(inc, l);
+                s = b + l;
+                start = __shfl(lo, l);
+                n_rows = __shfl(n, l) * group;
+                row0 = (int)(end - 1 - tile_id) * R;
+            } else before += __shfl(inc, 63);
+        }
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    if (s < 0) return;
+    row0 = __builtin_amdgcn_readfirstlane(row0); n_rows = __builtin_amdgcn_readfirstlane(n_rows); start = __builtin_amdgcn_readfirstlane(start);
+    const int past = p.lengths[s];
+    const int r = row0 + wave * 32 + l31, rr = min(r, n_rows - 1), tok = rr / group, h = kvh * group + rr - tok * group;
+    const int pos = past + tok;                                             // this lane's row sees keys up to here
+    const int wr_lo = min(row0 + wave * 32, n_rows - 1), wr_hi = min(row0 + wave * 32 + 31, n_rows - 1);
+    const int w_lo = past + wr_lo / group, w_hi = past + wr_hi / group;     // least and largest of the wave
+    const int b_lo = past + row0 / group, b_hi = past + (min(row0 + R, n_rows) - 1) / group;
+    int t_lo = 0, t_hi = b_hi < 0 ? 0 : b_hi / KT + 1;
+    if (a.splits > 1) {
+        const int per = (t_hi + a.splits - 1) / a.splits;
+        t_lo = min(t_hi, (int)blockIdx.y * per); t_hi = min(t_hi, t_lo + per);
+    }
+    // ---- Q fragments
+    u32x4 qf[TL::CPR / 2];
+    const T* q = (const T*)a.q + (int64_t)(start + tok) * a.q_sm + h * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < TL::CPR / 2; ++i) qf[i] = piece(q + (2 * i + hf) * TL::PER, (2 * i + hf) * TL::PER < Dh);
+    f32x16 acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    u32x4 kr[LD], vr[LD];
+    int pg[KT / 16], pn[KT / 16];                                           // pages of the 16-key groups: tile being loaded, the one after
+    auto pages = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i) pn[i] = t * KT + i * 16 <= b_hi ? paged_page(p, s, t * KT + i * 16) : -2;
+    };
+    auto load = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR, key = t * KT + row;
+            const int grp = __builtin_amdgcn_readfirstlane(row >> 4);       // a wave's 64 pieces lie in one group of 16 keys
+            int page = pg[0];
+#pragma unroll
+            for (int k = 1; k < KT / 16; ++k) page = grp == k ? pg[k] : page;
+            const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * Dh;
+            const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
+            const bool ok = page >= 0 && key <= b_hi;
+            kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
+            vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
+        }
+    };
+    auto bad_groups = [&]() { int b = 0;
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k) b |= (pg[k] == -1) << k;
+        return b; };
+    if (tid < 2) flag[tid] = 0;
+    int bad = 0, bad_next = 0;
+    if (t_lo < t_hi) {
+        pages(t_lo);
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k) pg[k] = pn[k];
+        load(t_lo);
+        bad_next = bad_groups();
+        pages(t_lo + 1);
+    }
+    __syncthreads();
+    for (int t = t_lo; t < t_hi; ++t) {
+        char* kt_lds = lds + ((t - t_lo) & 1) * 2 * TILE_BYTES;
+        char* vt_lds = kt_lds + TILE_BYTES;
+        const bool edge = t * KT + KT - 1 > b_lo;                           // some row of the block does not see the whole tile
+        unsigned long long* fl = flag + ((t - t_lo) & 1);
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            *(u32x4*)(kt_lds + (j * NT + tid) * 16) = kr[j];
+            *(u32x4*)(vt_lds + (j * NT + tid) * 16) = vr[j];
+        }
+        if (edge) {
+            // a value that is not finite would reach rows that do not see it (0 x NaN): remember which keys hold one
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                bool odd = false;
+#pragma unroll
+                for (int k = 0; k < TL::PER; ++k) {
+                    if constexpr (sizeof(T) == 4) odd |= !__builtin_isfinite(as<f32x4>(vr[j])[k]);
+                    else odd |= !__builtin_isfinite((float)as<V8>(vr[j])[k]);
+                }
+                if (odd) atomicOr(fl, 1ull << ((j * NT + tid) / TL::CPR));
+            }
+        }
+        bad = bad_next;
+        __syncthreads();
+        if (t + 1 < t_hi) {
+#pragma unroll
+            for (int k = 0; k < KT / 16; ++k) pg[k] = pn[k];
+            load(t + 1);
+            bad_next = bad_groups();
+            pages(t + 2);
+        }
+        if (edge && *fl) {                                                  // (uniform: read behind the barrier)
+            const unsigned long long keys = *fl;
+            for (int k = 0; k < KT; ++k) {
+                if (!(keys >> k & 1) || t * KT + k > pos) continue;
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const int d = i * 32 + 8 * (c >> 2) + 4 * hf + (c & 3);
+                        const float v = (float)*(const T*)(vt_lds + TL::voff(k, d / TL::PER) + d % TL::PER * (int)sizeof(T));
+                        if (!__builtin_isfinite(v)) acc[i][c] += v;         // whatever its weight, the sum is not finite
+                    }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < LD; ++j) {
+                char* at = vt_lds + (j * NT + tid) * 16;
+#pragma unroll
+                for (int k = 0; k < TL::PER; ++k)
+                    if (!__builtin_isfinite((float)((T*)at)[k])) ((T*)at)[k] = (T)0.f;
+            }
+            __syncthreads();
+            if (tid == 0) *fl = 0;
+        }
+        if (t * KT <= w_hi) {
+            f32x16 sc[NK];
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) sc[kt][c] = 0.f;
+#pragma unroll
+                for (int i = 0; i < TL::CPR / 2; ++i) {
+                    const u32x4 kf = *(const u32x4*)(kt_lds + TL::koff(kt * 32 + l31, 2 * i + hf));
+                    if constexpr (sizeof(T) == 2) sc[kt] = mma32(as<V8>(kf), as<V8>(qf[i]), sc[kt]);
+                    else
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) sc[kt] = mma32(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
+                }
+            }
+            if (bad) {
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        if (bad >> (kt * 2 + (c >> 3)) & 1) sc[kt][c] = NAN;
+            }
+            if (t * KT + KT - 1 > w_lo) {
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        sc[kt][c] = t * KT + kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= pos ? sc[kt][c] : -INFINITY;
+            }
+            float mt = sc[0][0];
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                for (int c = 0; c < 16; ++c) mt = fmaxf(mt, sc[kt][c]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32)) * a.scale_log2e;
+            if (__any(mt > m + LAZY)) {
+                const float mn = fmaxf(m, mt), al = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) acc[i][c] *= al;
+            }
+            const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                for (int c = 0; c < 16; ++c) { sc[kt][c] = exp2_hw(fmaf(sc[kt][c], a.scale_log2e, -ms)); l += sc[kt][c]; }
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int k16 = 0; k16 < KT / 16; ++k16) {
+                    V8 pf;                                                  // weights rounded to the tensors' type for the matrix instruction
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) pf[c] = (T)sc[k16 >> 1][(k16 & 1) * 8 + c];
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        const int row = k16 * 16 + 4 * hf + ((lane & 15) >> 2), c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), o = (lane & 1) * 8;
+                        s16x4 v[2] = {read_tr(vt_lds + TL::voff(row, c) + o), read_tr(vt_lds + TL::voff(row + 8, c) + o)};
+                        acc[i] = mma32(__builtin_bit_cast(V8, v), pf, acc[i]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const int row = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3);
+#pragma unroll
+                        for (int i = 0; i < DT; ++i)
+                            acc[i] = mma32(*(const float*)(vt_lds + TL::voff(row, 8 * i + (l31 >> 2)) + (l31 & 3) * 4), sc[kt][c], acc[i]);
+                    }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (r >= n_rows) return;
+    const int64_t orow = (int64_t)(start + tok) * p.Hq + h;
+    if (a.splits > 1) {
+        float* o = a.part + ((int64_t)blockIdx.y * p.M * p.Hq + orow) * (DP + 2);
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[i * 32 + 8 * (c >> 2) + 4 * hf + (c & 3)] = acc[i][c];
+        if (hf == 0) { o[DP] = m; o[DP + 1] = l; }
         return;
     }
-    for (int d = lane; d < Dh; d += 64) qs[d] = (float)((const T*)a.q)[m * a.q_sm + h * a.q_sh + d];
-    __syncthreads();
-    float mx = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int pmask = (1 << p.page_shift) - 1;
-    for (int64_t j0 = 0; j0 <= pos; j0 += 64) {
-        const int64_t j = j0 + lane;
-        float sc = -INFINITY;
-        int64_t base = -1;
-        if (j <= pos) {
-            const int pg = paged_page(p, s, (int)j);
-            if (pg >= 0) {
-                base = ((((int64_t)pg * p.Hkv + kvh) << p.page_shift) + (j & pmask)) * Dh;
-                float d0 = 0.f;
-                for (int d = 0; d < Dh; ++d) d0 += qs[d] * (float)((const T*)a.k_pages)[base + d];
-                sc = d0 * a.scale_log2e;
-            } else sc = NAN;
+    const float inv = 1.f / l;
+    T* o = (T*)a.out + orow * Dh;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+            const int d = i * 32 + 8 * c4 + 4 * hf;
+            typename Vec<T, 4>::type v;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = (T)(pos < 0 ? 0.f : acc[i][4 * c4 + c] * inv);
+            if (d < Dh) *(typename Vec<T, 4>::type*)(o + d) = v;
         }
-        float tm = sc;
-        for (int o = 32; o; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o));
-        const float mn = fmaxf(mx, tm), ms = mn == -INFINITY ? 0.f : mn;
-        const float pr = exp2f(sc - ms), al = exp2f(mx - ms);
-        float ts = pr;
-        for (int o = 32; o; o >>= 1) ts += __shfl_xor(ts, o);
-        l = l * al + ts;
-        mx = mn;
-        for (int k = 0; k < 4; ++k) acc[k] *= al;
-        ps[lane] = pr;
-        __syncthreads();
-        for (int i = 0; i < 64 && j0 + i <= pos; ++i) {
-            const int64_t b = ((int64_t)__shfl((int)(base >> 32), i) << 32) | (unsigned)__shfl((int)base, i);
-            if (b < 0) continue;
-            for (int k = 0; k < 4; ++k)
-                if (lane + 64 * k < Dh) acc[k] += ps[i] * (float)((const T*)a.v_pages)[b + lane + 64 * k];
-        }
-        __syncthreads();
+}
+
+// Adds the parts of a row's keys.  One wave per row and head.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
+    const PagedArgs& p = a.p;
+    const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (orow >= (int64_t)p.M * p.Hq) return;
+    const int lane = threadIdx.x & 63;
+    int pos;
+    const int s = paged_row(p, (int)(orow / p.Hq), pos);
+    T* out = (T*)a.out + orow * p.Dh;
+    if (s >= p.S || pos < 0) {
+        for (int d = lane; d < p.Dh; d += 64) out[d] = (T)0.f;
+        return;
     }
-    for (int k = 0; k < 4; ++k)
-        if (lane + 64 * k < Dh) out[lane + 64 * k] = (T)(acc[k] / l);
+    float M = -INFINITY, L = 0.f, acc[(DP + 63) / 64];
+#pragma unroll
+    for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = 0.f;
+    for (int i = 0; i < a.splits; ++i) {
+        const float* o = a.part + ((int64_t)i * p.M * p.Hq + orow) * (DP + 2);
+        const float m = o[DP], l = o[DP + 1], mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
+        const float ea = exp2_hw(M - ms), eb = exp2_hw(m - ms);
+#pragma unroll
+        for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = acc[k] * ea + o[min(lane + 64 * k, DP - 1)] * eb;
+        L = L * ea + l * eb;
+        M = mn;
+    }
+#pragma unroll
+    for (int k = 0; k < (DP + 63) / 64; ++k)
+        if (lane + 64 * k < p.Dh) out[lane + 64 * k] = (T)(acc[k] / L);
+}
+
+int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
+
+// Rows of a block: 32 per wave, as many as the streams have on average, fewer where the chip would not be filled
+int chunk_waves(const PagedArgs& p) {
+    const int64_t rows = (int64_t)p.M * (p.Hq / p.Hkv), per = rows / p.S;
+    const int64_t blocks8 = (rows / 256 + p.S) * p.Hkv;
+    return per > 128 && blocks8 >= 256 && padded_dim(p.Dh) <= 128 ? 8 : 4;
+}
+int64_t chunk_tiles(const PagedArgs& p, int nw) { return (int64_t)p.M * (p.Hq / p.Hkv) / (32 * nw) + p.S; }
+int chunk_splits(const PagedArgs& p, int elem, int nw) {
+    const int64_t blocks = chunk_tiles(p, nw) * p.Hkv, keys = (int64_t)p.width << p.page_shift;
+    int64_t s = blocks >= 512 ? 1 : 512 / blocks;
+    if (s > keys / 256) s = keys / 256;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+// a cache that cannot hold more than this is not worth a second launch
+bool one_whole(const PagedArgs& p) { return ((int64_t)p.width << p.page_shift) <= 512; }
+
+template <typename T, int DP> void run_one(AttendArgs a, hipStream_t s) {
+    const PagedArgs& p = a.p;
+    const int64_t segs = (int64_t)p.S * p.Hkv * ((p.Hq / p.Hkv + 15) / 16);
+    constexpr int keys = one_nw<DP>() * one_kt<T>();
+    a.splits = !one_whole(p);
+    attend_one<T, DP><<<a.splits ? ONE_GRID : (unsigned)segs, 64 * one_nw<DP>(), 0, s>>>(a);
+    if (a.splits) attend_join<T, DP><<<(unsigned)segs, DP, 0, s>>>(a, keys);
+}
+template <typename T, int DP, int NW> void run_chunk_nw(AttendArgs a, hipStream_t s) {
+    constexpr int bytes = 4 * chunk_kt<T>() * DP * (int)sizeof(T) + 64;
+    static bool set[64];                                        // per device: more LDS than a kernel gets by default
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (dev < 64 && !set[dev]) {
+        (void)hipFuncSetAttribute((const void*)attend_chunk<T, DP, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        set[dev] = true;
+    }
+    const dim3 grid((unsigned)(chunk_tiles(a.p, NW) * a.p.Hkv), (unsigned)a.splits);
+    attend_chunk<T, DP, NW><<<grid, 64 * NW, bytes, s>>>(a);
+    if (a.splits > 1) attend_chunk_join<T, DP><<<(unsigned)(((int64_t)a.p.M * a.p.Hq + 3) / 4), 256, 0, s>>>(a);
+}
+template <typename T, int DP> void run(AttendArgs a, int elem, hipStream_t s) {
+    if (!a.p.offsets) { run_one<T, DP>(a, s); return; }
+    const int nw = chunk_waves(a.p);
+    a.splits = chunk_splits(a.p, elem, nw);
+    if constexpr (DP <= 128) {
+        if (nw == 8) { run_chunk_nw<T, DP, 8>(a, s); return; }
+    }
+    run_chunk_nw<T, DP, 4>(a, s);
+}
+template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s) {
+    switch (padded_dim(a.p.Dh)) {
+        case 64: run<T, 64>(a, elem, s); break;
+        case 128: run<T, 128>(a, elem, s); break;
+        default: run<T, 256>(a, elem, s);
+    }
 }
 
 }  // namespace
 
-int64_t attend_workspace(const AttendArgs&, int) { return 0; }
+int64_t attend_workspace(const AttendArgs& a, int elem) {
+    const int DP = padded_dim(a.p.Dh);
+    if (!a.p.offsets) return one_whole(a.p) ? 0 : (int64_t)ONE_GRID * 2 * piece_floats(DP) * (int64_t)sizeof(float);
+    const int n = chunk_splits(a.p, elem, chunk_waves(a.p));
+    return n > 1 ? (int64_t)n * a.p.M * a.p.Hq * (DP + 2) * (int64_t)sizeof(float) : 0;
+}
 void launch_attend(AttendArgs a, int elem, hipStream_t s) {
-    const dim3 g(a.p.M, a.p.Hq);
-    if (elem == ELEM_F32) attend_rows<float><<<g, 64, 0, s>>>(a);
-    else if (elem == ELEM_F16) attend_rows<f16><<<g, 64, 0, s>>>(a);
-    else attend_rows<bfl><<<g, 64, 0, s>>>(a);
+    if (elem == ELEM_F32) run_dim<float>(a, elem, s);
+    else if (elem == ELEM_F16) run_dim<f16>(a, elem, s);
+    else run_dim<bfl>(a, elem, s);
 }

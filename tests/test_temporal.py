@@ -342,7 +342,8 @@ ATTEND = [
     ([2000, 5], [1, 1], 32, 4, 128, 64), ([700], [1], 5, 1, 80, 32), ([129, 64], [1, 1], 24, 3, 256, 128), ([4000], [1], 16, 1, 96, 1024),
     ([0], [33], 2, 1, 64, 16), ([0, 7, 40], [70, 0, 129], 8, 2, 128, 64), ([10, 200], [3, 2], 4, 4, 32, 16), ([-5, 90], [20, 40], 6, 2, 80, 32),
     ([1000], [65], 3, 3, 96, 128), ([0, 0, 0, 513], [1, 300, 2, 31], 4, 1, 64, 16), ([3000], [4], 8, 8, 128, 64), ([17], [260], 1, 1, 200, 16),
-    ([0] * 70, [3] * 70, 2, 2, 32, 16), ([250, -40, 3], [16, 16, 16], 16, 16, 40, 32),
+    ([100, 2000, 33], [1, 1, 1], 24, 1, 64, 16), ([5000, 0, 700], [1] * 3, 40, 2, 128, 64), ([900, 1200], [1, 1], 4, 4, 256, 256),
+    ([40], [50], 24, 1, 64, 32), ([0] * 70, [3] * 70, 2, 2, 32, 16), ([250, -40, 3], [16, 16, 16], 16, 16, 40, 32),
 ]
 
 
