@@ -158,8 +158,8 @@ typedef struct rvm_conv_args {
 int rvm_causal_conv(int dtype, const rvm_conv_args* args, void* hip_stream);
 
 /* delta = softplus(dt + dt_bias) (or dt + dt_bias with softplus = 0);  h_t = exp(delta_t * A) * h_(t-1) + delta_t * x_t * B_t;
- * y_t = sum_n C_t[n] h_t[n] + D * x_t, times z_t * sigmoid(z_t) where z is given.  State h [B,N,D] in fp32; state_out may be
- * state_in.  Workspace: rvm_selective_scan_workspace bytes (0: none), free for reuse when the call's work is done. */
+ * y_t = sum_n C_t[n] h_t[n] + D * x_t, times z_t * sigmoid(z_t) where z is given.  State h [B,N,D] in fp32; state_out must
+ * not overlap state_in.  Workspace: rvm_selective_scan_workspace bytes (0: none), free for reuse when the call's work is done. */
 typedef struct rvm_scan_args {
     const void *x, *dt, *z, *B, *C;             /* [B,T,D] x 3 (z may be NULL), [B,T,N] x 2, by strides */
     const float *A, *D, *dt_bias, *state_in;    /* [N,D]; [D], [D], [B,N,D] or NULL */

@@ -86,127 +86,192 @@ template <typename T, int VEC> void run_conv(const CausalConvArgs& a, hipStream_
 // One lane per channel with its N states in registers, a wave per 64 channels; B_t and C_t are the same for all channels and
 // come out of LDS as broadcasts (converted to fp32 once per wave and step, not once per channel).  The next steps' inputs are
 // requested before the present ones are worked on.
-// Where there are too few (sequence, 64 channels) pairs for the chip, the time axis is cut into chunks: ENDS computes each
-// chunk's last state from a zero start and the sum of its step sizes, scan_carry composes them (the decay over a chunk is
-// exp(A sum delta)) into every chunk's first state, and FROM runs the chunks from there.
+// Where there are too few (sequence, 64 channels) pairs for the chip, the time axis is cut into chunks, a wave each, the waves
+// of a block being neighbours.  ENDS computes each chunk's last state from a zero start and the sum of its step sizes, and
+// composes them over the block (the decay over a chunk is exp(A sum delta)): every chunk's first state within its block, and
+// the block's last.  FROM composes the blocks in front of it, then runs its chunks from there.
 enum ScanMode { SCAN_WHOLE, SCAN_ENDS, SCAN_FROM };
-constexpr int SCAN_WAVES = 4;
-template <int NP> constexpr int scan_batch() { return NP <= 16 ? 8 : 4; }
+constexpr int SCAN_WAVES = 8, SCAN_BATCH = 4;           // waves of a block where the time axis is cut; steps requested ahead
+template <int MODE> constexpr int scan_waves() { return MODE == SCAN_WHOLE ? 2 : SCAN_WAVES; }
+template <int NP> constexpr int scan_occupancy() { return NP <= 16 ? 4 : NP <= 32 ? 3 : 2; }      // waves of a SIMD
 
 template <typename T, int NP, int MODE>
-__global__ __launch_bounds__(64 * SCAN_WAVES) void selective_scan(ScanArgs a) {
-    constexpr int TB = scan_batch<NP>(), NV = MODE == SCAN_ENDS ? NP : 2 * NP, LD = (TB * NV + 63) / 64;
-    __shared__ __attribute__((aligned(16))) float bc_lds[SCAN_WAVES][2][LD * 64];
+__global__ __launch_bounds__(64 * scan_waves<MODE>(), scan_occupancy<NP>()) void selective_scan(ScanArgs a) {
+    constexpr int TB = SCAN_BATCH, NV = MODE == SCAN_ENDS ? NP : 2 * NP, LD = (TB * NV + 63) / 64, W = scan_waves<MODE>();
+    constexpr int BC = LD * 64, TAB = NP * 64;
+    constexpr int LDS = MODE == SCAN_ENDS ? (W * (TAB + 64) > W * 2 * BC ? W * (TAB + 64) : W * 2 * BC) : MODE == SCAN_FROM ? W * 2 * BC + TAB : W * 2 * BC;
+    __shared__ __attribute__((aligned(16))) float lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t unit = (int64_t)blockIdx.x * SCAN_WAVES + wave;
-    const int dti = (int)(unit % a.dtiles), ch = (int)(unit / a.dtiles % a.chunks);
-    const int64_t b = unit / a.dtiles / a.chunks;
-    if (b >= a.B) return;
+    const unsigned unit = MODE == SCAN_WHOLE ? blockIdx.x * W + wave : blockIdx.x;
+    const unsigned bq = unit / (unsigned)a.dtiles;
+    const int dti = (int)(unit - bq * (unsigned)a.dtiles), ch = MODE == SCAN_WHOLE ? 0 : blockIdx.y * W + wave;
+    const int64_t b = bq;
+    if (MODE == SCAN_WHOLE && b >= a.B) return;
     const int d_own = dti * 64 + lane, d = min(d_own, a.nD - 1);
     const bool own = d_own < a.nD;
-    const int t0 = MODE == SCAN_WHOLE ? 0 : ch * a.chunk_len, t1 = MODE == SCAN_WHOLE ? a.T : min(a.T, t0 + a.chunk_len);
-    const int64_t slot = (b * a.chunks + ch) * (int64_t)a.nD;
-    float h[NP], A2[NP];
-    const float* h0 = MODE == SCAN_WHOLE ? (a.state_in ? a.state_in + b * a.N * a.nD : nullptr) : MODE == SCAN_FROM ? a.carry + slot * a.N : nullptr;
-#pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        A2[n] = n < a.N ? a.A[(int64_t)n * a.nD + d] * LOG2E : 0.f;
-        h[n] = n < a.N && h0 ? h0[(int64_t)n * a.nD + d] : 0.f;
-    }
-    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
-    float steps = 0.f;
-    const T* x = (const T*)a.x + b * a.x_sb + d;
-    const T* dt = (const T*)a.dt + b * a.dt_sb + d;
-    const T* z = a.z ? (const T*)a.z + b * a.z_sb + d : nullptr;
-    const T* Bm = (const T*)a.Bm + b * a.B_sb;
-    const T* Cm = (const T*)a.Cm + b * a.C_sb;
-    T* y = (T*)a.y + b * a.T * a.nD + d;
+    const int t0 = MODE == SCAN_WHOLE ? 0 : min(a.T, ch * a.chunk_len), t1 = MODE == SCAN_WHOLE ? a.T : min(a.T, t0 + a.chunk_len);
+    const T* x = (const T*)a.x + b * a.x_sb + (int64_t)t0 * a.x_st + d;
+    const T* dt = (const T*)a.dt + b * a.dt_sb + (int64_t)t0 * a.dt_st + d;
+    const T* z = MODE != SCAN_ENDS && a.z ? (const T*)a.z + b * a.z_sb + (int64_t)t0 * a.z_st + d : nullptr;
+    const T* Bm = (const T*)a.Bm + b * a.B_sb + (int64_t)t0 * a.B_st;
+    const T* Cm = (const T*)a.Cm + b * a.C_sb + (int64_t)t0 * a.C_st;
     T xr[TB], dr[TB], zr[TB], br[LD];
-    auto load = [&](int t) {
+    auto load = [&](int left) {                         // the next `left` steps (TB or fewer: the last one again)
+        if (left >= TB) {
 #pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            const int64_t ti = min(t + i, t1 - 1);
-            xr[i] = x[ti * a.x_st];
-            dr[i] = dt[ti * a.dt_st];
-            if (MODE != SCAN_ENDS && z) zr[i] = z[ti * a.z_st];
+            for (int i = 0; i < TB; ++i) { xr[i] = x[i * a.x_st]; dr[i] = dt[i * a.dt_st]; }
+            if (z)
+#pragma unroll
+                for (int i = 0; i < TB; ++i) zr[i] = z[i * a.z_st];
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) { const int64_t k = min(i, left - 1); xr[i] = x[k * a.x_st]; dr[i] = dt[k * a.dt_st]; if (z) zr[i] = z[k * a.z_st]; }
         }
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
-            const int e = j * 64 + lane, v = e % NV, n = v % NP;
-            const int64_t ti = min(t + e / NV, t1 - 1);
-            br[j] = n < a.N ? (v < NP ? Bm[ti * a.B_st + n] : Cm[ti * a.C_st + n]) : (T)0.f;
+            const int e = j * 64 + lane, v = e % NV, n = min(v % NP, a.N - 1);
+            const int64_t k = min(e / NV, left - 1);
+            br[j] = v < NP ? Bm[k * a.B_st + n] : Cm[k * a.C_st + n];
         }
+        x += TB * a.x_st; dt += TB * a.dt_st; Bm += TB * a.B_st; Cm += TB * a.C_st;
+        if (z) z += TB * a.z_st;
     };
-    if (t0 < t1) load(t0);
+    if (t0 < t1) load(t1 - t0);
+    // ---- first states.  States past N: decay 1, input 0, start 0 - they stay 0
+    float h[NP], A2[NP];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) A2[n] = a.A[(int64_t)min(n, a.N - 1) * a.nD + d];
+    const float* first = a.state_in ? a.state_in + b * a.N * a.nD : nullptr;
+    const int64_t slot = (b * a.chunks + ch) * (int64_t)a.nD;           // of this chunk in carry and steps
+    float steps = 0.f;
+    if (MODE == SCAN_FROM) {
+        // the block's first state: a thread takes (n, channel) pairs and composes the blocks in front, eight requests at a time
+        float* H = lds + W * 2 * BC;
+        const int64_t per = (int64_t)a.nD * (a.N + 1);
+        const float* tot = a.totals + (b * gridDim.y) * per + d;        // per block: N rows of last states, a row of step sums
+        for (int n = wave; n < NP; n += W) {
+            const int nn = min(n, a.N - 1);
+            const float A2n = a.A[(int64_t)nn * a.nD + d] * LOG2E;
+            float hb = first ? first[(int64_t)nn * a.nD + d] : 0.f;
+            constexpr int U = 8;
+            for (int k0 = 0; k0 < (int)blockIdx.y; k0 += U) {
+                float e[U], st[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const float* at = tot + min(k0 + k, (int)blockIdx.y - 1) * per;
+                    e[k] = at[(int64_t)nn * a.nD]; st[k] = at[(int64_t)a.N * a.nD];
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (k0 + k < (int)blockIdx.y) hb = fmaf(exp2_hw(st[k] * A2n), hb, e[k]);
+            }
+            H[n * 64 + lane] = hb;
+        }
+        const float before = a.steps[slot + d];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) h[n] = a.carry[slot * a.N + (int64_t)min(n, a.N - 1) * a.nD + d];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            A2[n] = n < a.N ? A2[n] * LOG2E : 0.f;
+            h[n] = n < a.N ? fmaf(exp2_hw(A2[n] * before), H[n * 64 + lane], h[n]) : 0.f;
+        }
+    } else {
+        if (MODE == SCAN_WHOLE && first) {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) h[n] = first[(int64_t)min(n, a.N - 1) * a.nD + d];
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) h[n] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            A2[n] = n < a.N ? A2[n] * LOG2E : 0.f;
+            h[n] = n < a.N ? h[n] : 0.f;
+        }
+    }
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
+    T* y = (T*)a.y + (b * a.T + t0) * a.nD + d;
     int buf = 0;
     for (int t = t0; t < t1; t += TB, buf ^= 1) {
-        float* bc = bc_lds[wave][buf];
+        float* bc = lds + (wave * 2 + buf) * BC;
         float xv[TB], dv[TB], zv[TB];
 #pragma unroll
-        for (int i = 0; i < TB; ++i) { xv[i] = (float)xr[i]; dv[i] = (float)dr[i] + bias; if (MODE != SCAN_ENDS && z) zv[i] = (float)zr[i]; }
+        for (int i = 0; i < TB; ++i) { xv[i] = (float)xr[i]; dv[i] = (float)dr[i] + bias; if (MODE != SCAN_ENDS) zv[i] = z ? (float)zr[i] : 0.f; }
 #pragma unroll
-        for (int j = 0; j < LD; ++j) bc[j * 64 + lane] = (float)br[j];
-        if (t + TB < t1) load(t + TB);
+        for (int j = 0; j < LD; ++j) bc[j * 64 + lane] = (j * 64 + lane) % NP < a.N ? (float)br[j] : 0.f;
+        if (t + TB < t1) load(t1 - t - TB);
+        if (a.softplus)
 #pragma unroll
-        for (int i = 0; i < TB; ++i)
-            if (t + i < t1) {
-                const float delta = a.softplus ? softplus_f(dv[i]) : dv[i], dx = delta * xv[i];
-                float o = MODE == SCAN_ENDS ? 0.f : skip * xv[i];
-                if (MODE == SCAN_ENDS) steps += delta;
+            for (int i = 0; i < TB; ++i) dv[i] = softplus_f(dv[i]);
+        auto step = [&](int i) {
+            const float delta = dv[i], dx = delta * xv[i];
+            float o = MODE == SCAN_ENDS ? 0.f : skip * xv[i];
+            if (MODE == SCAN_ENDS) steps += delta;
 #pragma unroll
-                for (int n4 = 0; n4 < NP; n4 += 4) {
-                    const f32x4 bv = *(const f32x4*)(bc + i * NV + n4);
-                    f32x4 cv;
-                    if (MODE != SCAN_ENDS) cv = *(const f32x4*)(bc + i * NV + NP + n4);
+            for (int n4 = 0; n4 < NP; n4 += 4) {
+                const f32x4 bv = *(const f32x4*)(bc + i * NV + n4);
+                f32x4 cv;
+                if (MODE != SCAN_ENDS) cv = *(const f32x4*)(bc + i * NV + NP + n4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        h[n4 + k] = fmaf(exp2_hw(delta * A2[n4 + k]), h[n4 + k], dx * bv[k]);
-                        if (MODE != SCAN_ENDS) o = fmaf(h[n4 + k], cv[k], o);
-                    }
-                }
-                if (MODE != SCAN_ENDS) {
-                    if (z) o *= silu_f(zv[i]);
-                    if (own) y[(int64_t)(t + i) * a.nD] = (T)o;
+                for (int k = 0; k < 4; ++k) {
+                    h[n4 + k] = fmaf(exp2_hw(delta * A2[n4 + k]), h[n4 + k], dx * bv[k]);
+                    if (MODE != SCAN_ENDS) o = fmaf(h[n4 + k], cv[k], o);
                 }
             }
+            if (MODE != SCAN_ENDS) {
+                if (z) o *= silu_f(zv[i]);
+                if (own) y[(int64_t)(t - t0 + i) * a.nD] = (T)o;
+            }
+        };
+        if (t + TB <= t1) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) { step(i); __builtin_amdgcn_sched_barrier(0); }      // (steps side by side cost registers, i.e. waves)
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB; ++i)
+                if (t + i < t1) step(i);
+        }
     }
-    if (!own || MODE == SCAN_FROM) return;
-    float* out = MODE == SCAN_WHOLE ? a.state_out + b * a.N * a.nD : a.carry + slot * a.N;
+    if (MODE == SCAN_ENDS) {
+        float* S = lds + W * TAB;                       // (the B values are done with)
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NP; ++n) lds[wave * TAB + n * 64 + lane] = h[n];
+        S[wave * 64 + lane] = steps;
+        __syncthreads();
+        float* tot = a.totals + (b * gridDim.y + blockIdx.y) * (int64_t)a.nD * (a.N + 1) + d;
+        const int64_t slot0 = (b * a.chunks + blockIdx.y * W) * (int64_t)a.nD;
+        for (int n = wave; n < a.N; n += W) {
+            const float A2n = a.A[(int64_t)n * a.nD + d] * LOG2E;
+            float hb = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (own) a.carry[(slot0 + (int64_t)w * a.nD) * a.N + (int64_t)n * a.nD + d] = hb;
+                hb = fmaf(exp2_hw(A2n * S[w * 64 + lane]), hb, lds[w * TAB + n * 64 + lane]);
+            }
+            if (own) tot[(int64_t)n * a.nD] = hb;
+        }
+        float sum = 0.f;
+        for (int w = 0; w < wave; ++w) sum += S[w * 64 + lane];
+        if (own) a.steps[slot + d] = sum;
+        if (own && wave == W - 1) tot[(int64_t)a.N * a.nD] = sum + steps;
+        return;
+    }
+    if (!own || (MODE == SCAN_FROM && ch != a.chunks - 1)) return;
+    float* out = a.state_out + b * a.N * a.nD;
 #pragma unroll
     for (int n = 0; n < NP; ++n)
         if (n < a.N) out[(int64_t)n * a.nD + d] = h[n];
-    if (MODE == SCAN_ENDS) a.steps[slot + d] = steps;
-}
-
-// every chunk's first state in place of its last one, and the sequence's last state
-__global__ __launch_bounds__(256) void scan_carry(ScanArgs a) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)a.N * a.nD, b = id / per;
-    if (b >= a.B) return;
-    const int64_t nd = id - b * per;
-    const int d = (int)(nd % a.nD);
-    const float A2 = a.A[nd] * LOG2E;
-    float h = a.state_in ? a.state_in[id] : 0.f;
-    float* c = a.carry + b * a.chunks * per + nd;
-    const float* st = a.steps + b * a.chunks * a.nD + d;
-    constexpr int U = 8;
-    for (int i = 0; i < a.chunks; i += U) {
-        float e[U], s[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) { const int64_t j = min(i + k, a.chunks - 1); e[k] = c[j * per]; s[k] = st[j * a.nD]; }
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (i + k < a.chunks) { c[(i + k) * per] = h; h = fmaf(exp2_hw(s[k] * A2), h, e[k]); }
-    }
-    a.state_out[id] = h;
 }
 
 template <typename T, int NP> void run_scan_n(const ScanArgs& a, hipStream_t s) {
-    const int64_t units = (int64_t)a.B * a.dtiles * a.chunks;
-    const unsigned g = (unsigned)((units + SCAN_WAVES - 1) / SCAN_WAVES);
-    if (a.chunks == 1) { selective_scan<T, NP, SCAN_WHOLE><<<g, 64 * SCAN_WAVES, 0, s>>>(a); return; }
-    selective_scan<T, NP, SCAN_ENDS><<<g, 64 * SCAN_WAVES, 0, s>>>(a);
-    scan_carry<<<(unsigned)(((int64_t)a.B * a.N * a.nD + 255) / 256), 256, 0, s>>>(a);
-    selective_scan<T, NP, SCAN_FROM><<<g, 64 * SCAN_WAVES, 0, s>>>(a);
+    constexpr int W = SCAN_WAVES, WW = scan_waves<SCAN_WHOLE>();
+    const unsigned units = (unsigned)(a.B * a.dtiles);
+    if (a.chunks == 1) { selective_scan<T, NP, SCAN_WHOLE><<<(units + WW - 1) / WW, 64 * WW, 0, s>>>(a); return; }
+    const dim3 grid(units, (unsigned)(a.chunks / W));
+    selective_scan<T, NP, SCAN_ENDS><<<grid, 64 * W, 0, s>>>(a);
+    selective_scan<T, NP, SCAN_FROM><<<grid, 64 * W, 0, s>>>(a);
 }
 template <typename T> void run_scan(const ScanArgs& a, hipStream_t s) {
     if (a.N <= 8) run_scan_n<T, 8>(a, s);
@@ -230,19 +295,24 @@ void launch_causal_conv(const CausalConvArgs& a0, int elem, hipStream_t s) {
     else { if (wide) run_conv<bfl, 8>(a, s); else run_conv<bfl, 1>(a, s); }
 }
 
-// Chunks of the time axis: none where every SIMD has a wave without them, otherwise as many as give it four, of 32 steps at least
+// Chunks of the time axis, a multiple of a block's waves: none where every SIMD has a wave without them, otherwise as many as
+// give it four waves (what the registers allow), of 16 steps at least
 int scan_chunks(int B, int T, int D) {
-    const int64_t waves = (int64_t)B * ((D + 63) / 64);
+    const int64_t waves = (int64_t)B * ((D + 63) / 64), W = SCAN_WAVES;
     if (waves >= 1024 || T < 64) return 1;
-    int64_t n = (4096 + waves - 1) / waves;
-    if (n > T / 32) n = T / 32;
-    const int len = (int)((T + n - 1) / n + 7) / 8 * 8;
-    return (T + len - 1) / len;
+    int64_t n = 4096 / waves / W * W;
+    if (n > T / 16 / W * W) n = T / 16 / W * W;
+    return n < W ? (T < 16 * W ? 1 : (int)W) : (int)n;
+}
+int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N) {
+    return B * (chunks + chunks / SCAN_WAVES) * (N + 1) * D;
 }
 void launch_selective_scan(const ScanArgs& a0, int elem, hipStream_t s) {
     ScanArgs a = a0;
     a.dtiles = (a.nD + 63) / 64;
     a.chunk_len = a.chunks > 1 ? ((a.T + a.chunks - 1) / a.chunks + 7) / 8 * 8 : a.T;
+    a.steps = a.carry + (int64_t)a.B * a.chunks * a.N * a.nD;
+    a.totals = a.steps + (int64_t)a.B * a.chunks * a.nD;
     if (elem == ELEM_F32) run_scan<float>(a, s);
     else if (elem == ELEM_F16) run_scan<f16>(a, s);
     else run_scan<bfl>(a, s);

@@ -69,7 +69,7 @@ int64_t rvm_selective_scan_workspace(int64_t B, int64_t T, int64_t D, int64_t N)
     if (B < 0 || T < 0 || D < 0 || N < 1 || B > INT_LIMIT || T > INT_LIMIT || D > INT_LIMIT || N > 64) return -1;
     if (!B || !D) return 0;
     const int64_t chunks = scan_chunks((int)B, (int)T, (int)D);
-    return chunks > 1 ? B * chunks * (N + 1) * D * (int64_t)sizeof(float) : 0;
+    return chunks > 1 ? scan_workspace_floats(B, chunks, D, N) * (int64_t)sizeof(float) : 0;
 }
 
 int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
@@ -82,6 +82,7 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
     if (!c->nB || !c->nD) return 0;
     if (!c->A || !c->state_out || (c->nT && (!c->x || !c->dt || !c->B || !c->C || !c->y))) return fail(who, "null buffer");
     if ((double)c->nB * ((c->nD + 63) / 64) > 1e9) return fail(who, "too large for one launch");
+    if (c->state_in == c->state_out) return fail(who, "state_out must not alias state_in");
     const int64_t need = rvm_selective_scan_workspace(c->nB, c->nT, c->nD, c->nN);
     if (need > 0 && (!c->workspace || c->workspace_bytes < need)) return fail(who, "workspace too small (rvm_selective_scan_workspace)");
     ScanArgs a; memset(&a, 0, sizeof a);
@@ -92,7 +93,6 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
     a.B = (int)c->nB; a.T = (int)c->nT; a.nD = (int)c->nD; a.N = (int)c->nN; a.softplus = c->softplus != 0;
     a.chunks = scan_chunks(a.B, a.T, a.nD);
     a.carry = (float*)c->workspace;
-    if (a.carry) a.steps = a.carry + (int64_t)a.B * a.chunks * a.N * a.nD;
     launch_selective_scan(a, elem, (hipStream_t)hip_stream);
     return launched(who);
 }

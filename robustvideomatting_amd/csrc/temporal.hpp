@@ -22,12 +22,13 @@ struct ScanArgs {
     const void *x, *dt, *z, *Bm, *Cm;                   // z may be null
     const float *A, *D, *dt_bias, *state_in;            // [N,D]; the other three may be null
     void* y; float* state_out;                          // [B,T,D], [B,N,D]
-    float *carry, *steps;                               // time split: [B][chunks][N][D] states, [B][chunks][D] sums of step sizes
+    float *carry, *steps, *totals;                      // time split: [B][chunks][N][D] states, [B][chunks][D] sums of step sizes, of blocks
     int64_t x_sb, x_st, dt_sb, dt_st, z_sb, z_st, B_sb, B_st, C_sb, C_st;
     int B, T, nD, N, softplus, chunks, chunk_len, dtiles;
 };
 // how the time axis is split for this shape (1: not at all)
 int scan_chunks(int B, int T, int D);
+int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N);
 void launch_selective_scan(const ScanArgs& a, int elem, hipStream_t s);
 
 // A stream's cache: position p lives in page table[s][p / page], slot p % page, of the pools [pages][Hkv][page][Dh]

@@ -73,6 +73,8 @@ ATTEND_OK = dict(q=4096, k_pages=4096, v_pages=4096, out=4096, workspace=0, tabl
     ("rvm_selective_scan", SCAN_OK, dict(nN=0), "states"),
     ("rvm_selective_scan", SCAN_OK, dict(nN=65), "states"),
     ("rvm_selective_scan", SCAN_OK, dict(A=0), "null"),
+    ("rvm_selective_scan", SCAN_OK, dict(state_in=4096), "alias"),
+    ("rvm_selective_scan", SCAN_OK, dict(nT=4096), "workspace"),
     ("rvm_selective_scan", SCAN_OK, dict(nD=-8), "shape"),
     ("rvm_append_kv", APPEND_OK, dict(Hq=3), "multiple"),
     ("rvm_append_kv", APPEND_OK, dict(Dh=20), "head size"),
