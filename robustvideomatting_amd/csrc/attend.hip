@@ -153,34 +153,37 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
         float m = -INFINITY, l = 0.f;
         bool lost = false;
         u32x4 kr[LD], vr[LD];
-        int pg[2];
-        auto pages = [&](int t) {
-            const int k0 = t * KT;
-            pg[0] = k0 <= pos ? paged_page(p, s, k0) : -2;
-            if (KT > 16) pg[1] = k0 + 16 <= pos ? paged_page(p, s, k0 + 16) : -2;
-            lost |= pg[0] == -1 || (KT > 16 && pg[1] == -1);
+        // page numbers of a tile's groups of 16 keys, looked up a tile before they are used and by vector loads (each lane a
+        // key of the group): a scalar load would be waited for together with the LDS reads
+        int entry[KT / 16];
+        const int* table = p.table + (int64_t)s * p.width;
+        const int page_mask = (1 << p.page_shift) - 1;
+        auto look = [&](int t) {
+#pragma unroll
+            for (int k = 0; k < KT / 16; ++k) entry[k] = table[min(((unsigned)t * KT + k * 16 + l15) >> p.page_shift, (unsigned)p.width - 1)];
         };
         auto load = [&](int t) {
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
-                const int i = j * 64 + lane, row = i / TL::CPR, pc = i % TL::CPR, key = t * KT + row;
-                const int page = KT > 16 && row >= 16 ? pg[1] : pg[0];
-                const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * Dh;
+                const int i = j * 64 + lane, row = i / TL::CPR, pc = i % TL::CPR, page = entry[KT > 16 ? j * 64 / TL::CPR >> 4 : 0];
+                const unsigned key = (unsigned)t * KT + row;
+                const bool here = (unsigned)page < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width, ok = here && key <= (unsigned)pos;
+                lost |= !here && key <= (unsigned)pos;
+                const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
                 const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
-                const bool ok = page >= 0 && key <= pos;
                 kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
                 vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
             }
         };
         int t = ua * NW + wave;
-        if (t < t_end) { pages(t); load(t); if (t + NW < t_end) pages(t + NW); }
+        if (t < t_end) { look(t); load(t); look(t + NW); }
         for (; t < t_end; t += NW) {
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
                 *(u32x4*)(kt_lds + (j * 64 + lane) * 16) = kr[j];
                 *(u32x4*)(vt_lds + (j * 64 + lane) * 16) = vr[j];
             }
-            if (t + NW < t_end) { load(t + NW); if (t + 2 * NW < t_end) pages(t + 2 * NW); }
+            if (t + NW < t_end) { load(t + NW); look(t + 2 * NW); }
             // ---- scores: lane = (row l15, keys 4 g .. 4 g + 3 of each 16)
             f32x4 sc[KT / 16];
 #pragma unroll
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float v = sc[kt][c] * a.scale_log2e;
-                    sc[kt][c] = t * KT + kt * 16 + 4 * g + c <= pos ? v : -INFINITY;
+                    sc[kt][c] = kt * 16 + 4 * g + c <= pos - t * KT ? v : -INFINITY;
                     mt = fmaxf(mt, sc[kt][c]);
                 }
             mt = fmaxf(mt, __shfl_xor(mt, 16));
@@ -319,7 +322,8 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     constexpr int LD = KT * TL::CPR / NT, TILE_BYTES = KT * TL::PITCH;
     typedef typename Vec<T, 8>::type V8;
     extern __shared__ __attribute__((aligned(16))) char lds[];              // two buffers of a K and a V tile, flags
-    unsigned long long* flag = (unsigned long long*)(lds + 4 * TILE_BYTES); // [2]: rows of a V tile that are not finite
+    unsigned long long* flag = (unsigned long long*)(lds + 4 * TILE_BYTES); // [3]: rows of a V tile that are not finite
+    int* badf = (int*)(flag + 3);                                           // [3]: groups of 16 keys without a page
     const PagedArgs& p = a.p;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, hf = lane >> 5;
     const int group = p.Hq / p.Hkv, Dh = p.Dh;
@@ -360,11 +364,12 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     if (s < 0) return;
     row0 = __builtin_amdgcn_readfirstlane(row0); n_rows = __builtin_amdgcn_readfirstlane(n_rows); start = __builtin_amdgcn_readfirstlane(start);
     const int past = p.lengths[s];
+    auto at = [&](int token) { return (int)min((int64_t)INT32_MAX, max((int64_t)-1, (int64_t)past + token)); };
     const int r = row0 + wave * 32 + l31, rr = min(r, n_rows - 1), tok = rr / group, h = kvh * group + rr - tok * group;
-    const int pos = past + tok;                                             // this lane's row sees keys up to here
+    const int pos = at(tok);                                                // this lane's row sees keys up to here
     const int wr_lo = min(row0 + wave * 32, n_rows - 1), wr_hi = min(row0 + wave * 32 + 31, n_rows - 1);
-    const int w_lo = past + wr_lo / group, w_hi = past + wr_hi / group;     // least and largest of the wave
-    const int b_lo = past + row0 / group, b_hi = past + (min(row0 + R, n_rows) - 1) / group;
+    const int w_lo = at(wr_lo / group), w_hi = at(wr_hi / group);           // least and largest of the wave
+    const int b_lo = at(row0 / group), b_hi = at((min(row0 + R, n_rows) - 1) / group);
     int t_lo = 0, t_hi = b_hi < 0 ? 0 : b_hi / KT + 1;
     if (a.splits > 1) {
         const int per = (t_hi + a.splits - 1) / a.splits;
@@ -382,46 +387,38 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
         for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
     float m = -INFINITY, l = 0.f;
     u32x4 kr[LD], vr[LD];
-    int pg[KT / 16], pn[KT / 16];                                           // pages of the 16-key groups: tile being loaded, the one after
-    auto pages = [&](int t) {
+    // Page numbers are looked up a tile before they are used, each thread those of its own rows, and by vector loads: a scalar
+    // load would be waited for together with the LDS reads.  entry[j]: what the table holds for the tile to be requested next
+    int entry[LD];
+    bool lost = false;                                                      // a row of mine in the tile requested last has no page
+    const int page_mask = (1 << p.page_shift) - 1;
+    const int* table = p.table + (int64_t)s * p.width;
+    auto look = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < KT / 16; ++i) pn[i] = t * KT + i * 16 <= b_hi ? paged_page(p, s, t * KT + i * 16) : -2;
+        for (int j = 0; j < LD; ++j) entry[j] = table[min(((unsigned)t * KT + (j * NT + tid) / TL::CPR) >> p.page_shift, (unsigned)p.width - 1)];
     };
     auto load = [&](int t) {
+        lost = false;
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
-            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR, key = t * KT + row;
-            const int grp = __builtin_amdgcn_readfirstlane(row >> 4);       // a wave's 64 pieces lie in one group of 16 keys
-            int page = pg[0];
-#pragma unroll
-            for (int k = 1; k < KT / 16; ++k) page = grp == k ? pg[k] : page;
-            const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * Dh;
+            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR;
+            const unsigned key = (unsigned)t * KT + row;
+            const bool here = (unsigned)entry[j] < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width, ok = here && key <= (unsigned)b_hi;
+            lost |= !here && key <= (unsigned)b_hi;
+            const int64_t base = ((((int64_t)entry[j] * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
             const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
-            const bool ok = page >= 0 && key <= b_hi;
             kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
             vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
         }
     };
-    auto bad_groups = [&]() { int b = 0;
-#pragma unroll
-        for (int k = 0; k < KT / 16; ++k) b |= (pg[k] == -1) << k;
-        return b; };
-    if (tid < 2) flag[tid] = 0;
-    int bad = 0, bad_next = 0;
-    if (t_lo < t_hi) {
-        pages(t_lo);
-#pragma unroll
-        for (int k = 0; k < KT / 16; ++k) pg[k] = pn[k];
-        load(t_lo);
-        bad_next = bad_groups();
-        pages(t_lo + 1);
-    }
+    if (tid < 3) { flag[tid] = 0; badf[tid] = 0; }
+    if (t_lo < t_hi) { look(t_lo); load(t_lo); look(t_lo + 1); }
     __syncthreads();
     for (int t = t_lo; t < t_hi; ++t) {
         char* kt_lds = lds + ((t - t_lo) & 1) * 2 * TILE_BYTES;
         char* vt_lds = kt_lds + TILE_BYTES;
-        const bool edge = t * KT + KT - 1 > b_lo;                           // some row of the block does not see the whole tile
-        unsigned long long* fl = flag + ((t - t_lo) & 1);
+        const bool edge = b_lo - t * KT < KT - 1;                           // some row of the block does not see the whole tile
+        const int slot = (t - t_lo) % 3;                                    // flags are cleared two barriers before they are used again
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
             *(u32x4*)(kt_lds + (j * NT + tid) * 16) = kr[j];
@@ -437,22 +434,24 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
                     if constexpr (sizeof(T) == 4) odd |= !__builtin_isfinite(as<f32x4>(vr[j])[k]);
                     else odd |= !__builtin_isfinite((float)as<V8>(vr[j])[k]);
                 }
-                if (odd) atomicOr(fl, 1ull << ((j * NT + tid) / TL::CPR));
+                if (odd) atomicOr(flag + slot, 1ull << ((j * NT + tid) / TL::CPR));
             }
         }
-        bad = bad_next;
-        __syncthreads();
-        if (t + 1 < t_hi) {
+        if (__any(lost)) {                                                  // (a page holds 16 keys or more: a group has one or none)
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k) pg[k] = pn[k];
-            load(t + 1);
-            bad_next = bad_groups();
-            pages(t + 2);
+            for (int j = 0; j < LD; ++j) {
+                const unsigned row = (j * NT + tid) / TL::CPR, col = ((unsigned)t * KT + row) >> p.page_shift;
+                if (t * KT + row <= (unsigned)b_hi && (col >= (unsigned)p.width || (unsigned)table[col] >= (unsigned)p.pages)) atomicOr(badf + slot, 1 << (row >> 4));
+            }
         }
-        if (edge && *fl) {                                                  // (uniform: read behind the barrier)
-            const unsigned long long keys = *fl;
+        __syncthreads();
+        const int bad = badf[slot];
+        if (tid == 0) { const int next = slot == 0 ? 2 : slot - 1; flag[next] = 0; badf[next] = 0; }
+        if (t + 1 < t_hi) { load(t + 1); look(t + 2); }
+        const unsigned long long keys = edge ? flag[slot] : 0;
+        if (keys) {
             for (int k = 0; k < KT; ++k) {
-                if (!(keys >> k & 1) || t * KT + k > pos) continue;
+                if (!(keys >> k & 1) || pos - t * KT < k) continue;
 #pragma unroll
                 for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -471,36 +470,36 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
                     if (!__builtin_isfinite((float)((T*)at)[k])) ((T*)at)[k] = (T)0.f;
             }
             __syncthreads();
-            if (tid == 0) *fl = 0;
         }
         if (t * KT <= w_hi) {
             f32x16 sc[NK];
 #pragma unroll
-            for (int kt = 0; kt < NK; ++kt) {
+            for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                 for (int c = 0; c < 16; ++c) sc[kt][c] = 0.f;
 #pragma unroll
-                for (int i = 0; i < TL::CPR / 2; ++i) {
+            for (int i = 0; i < TL::CPR / 2; ++i)
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt) {
                     const u32x4 kf = *(const u32x4*)(kt_lds + TL::koff(kt * 32 + l31, 2 * i + hf));
                     if constexpr (sizeof(T) == 2) sc[kt] = mma32(as<V8>(kf), as<V8>(qf[i]), sc[kt]);
                     else
 #pragma unroll
                         for (int c = 0; c < 4; ++c) sc[kt] = mma32(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
                 }
-            }
-            if (bad) {
+            if (bad) {                                                      // scores of keys without a page: not a number
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
                         if (bad >> (kt * 2 + (c >> 3)) & 1) sc[kt][c] = NAN;
             }
-            if (t * KT + KT - 1 > w_lo) {
+            if (w_lo - t * KT < KT - 1) {
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
-                        sc[kt][c] = t * KT + kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= pos ? sc[kt][c] : -INFINITY;
+                        sc[kt][c] = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= pos - t * KT ? sc[kt][c] : -INFINITY;
             }
             float mt = sc[0][0];
 #pragma unroll
