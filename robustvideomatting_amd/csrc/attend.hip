@@ -45,10 +45,11 @@ __device__ __forceinline__ f32x16 mma32(b16x8 a, b16x8 b, f32x16 c) { return __b
 __device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
 template <typename V> __device__ __forceinline__ V as(u32x4 v) { return __builtin_bit_cast(V, v); }
+// What is not there is read from here: a choice of addresses instead of a branch per load, behind which the compiler loses
+// count of the loads in flight and waits for all of them
+__device__ const u32x4 zero_piece = {0, 0, 0, 0};
 template <typename T> __device__ __forceinline__ u32x4 piece(const T* p, bool ok) {
-    u32x4 z = {0, 0, 0, 0};
-    if (ok) z = *(const u32x4*)p;
-    return z;
+    return *(ok ? (const u32x4*)p : &zero_piece);
 }
 
 // ---- one token per stream -------------------------------------------------------------------------------------------------
@@ -399,16 +400,25 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     };
     auto load = [&](int t) {
         lost = false;
+        const T *kp[LD], *vp[LD];                                           // (all page numbers are used before a load is issued)
+        bool ok[LD];
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
             const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR;
             const unsigned key = (unsigned)t * KT + row;
-            const bool here = (unsigned)entry[j] < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width, ok = here && key <= (unsigned)b_hi;
+            const bool here = (unsigned)entry[j] < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width;
+            ok[j] = here && key <= (unsigned)b_hi;
             lost |= !here && key <= (unsigned)b_hi;
             const int64_t base = ((((int64_t)entry[j] * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
-            const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
-            kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
-            vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
+            kp[j] = (const T*)a.k_pages + base + TL::kswz(row, pc) * TL::PER;
+            vp[j] = (const T*)a.v_pages + base + TL::vswz(row, pc) * TL::PER;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < LD; ++j) {
+            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR;
+            kr[j] = piece(kp[j], ok[j] && TL::kswz(row, pc) * TL::PER < Dh);
+            vr[j] = piece(vp[j], ok[j] && TL::vswz(row, pc) * TL::PER < Dh);
         }
     };
     if (tid < 3) { flag[tid] = 0; badf[tid] = 0; }
@@ -445,7 +455,6 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
             }
         }
         __syncthreads();
-        const int bad = badf[slot];
         if (tid == 0) { const int next = slot == 0 ? 2 : slot - 1; flag[next] = 0; badf[next] = 0; }
         if (t + 1 < t_hi) { load(t + 1); look(t + 2); }
         const unsigned long long keys = edge ? flag[slot] : 0;
@@ -472,6 +481,7 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
             __syncthreads();
         }
         if (t * KT <= w_hi) {
+            const int bad = badf[slot];
             f32x16 sc[NK];
 #pragma unroll
             for (int kt = 0; kt < NK; ++kt)
