@@ -23,13 +23,14 @@ template <typename T, int DP> struct Tile {
     static constexpr int PER = 16 / (int)sizeof(T), CPR = DP / PER, RPL = CPR >= 16 ? 1 : 16 / CPR, PITCH = DP * (int)sizeof(T);
     // keys: 16 rows, the same piece of each
     __device__ static __forceinline__ int kswz(int row, int c) { return c ^ ((row / RPL) & (CPR < 16 ? CPR - 1 : 15)); }
-    // values, 16-bit: 8 rows, the same two pieces of each (transposing read); fp32: rows 4 apart, the same four (or eight)
-    __device__ static __forceinline__ int vswz(int row, int c) {
-        if constexpr (sizeof(T) == 2) return c ^ (((row / RPL) << 1) & (CPR < 16 ? CPR - 1 : 15));
+    // values, 16-bit (transposing read, 32 lanes at a time): 8 rows, the same two pieces of each (MF = 16 x 16 tiles), or
+    // 4 rows, the same four pieces (MF = 32); fp32: rows 4 apart, the same four (or eight)
+    template <int MF> __device__ static __forceinline__ int vswz(int row, int c) {
+        if constexpr (sizeof(T) == 2) return c ^ (((row / RPL) << (MF == 16 ? 1 : 2)) & (CPR < 16 ? CPR - 1 : 15));
         else return c ^ ((((row >> 2) & 3) << 2) & (CPR - 1));
     }
     __device__ static __forceinline__ int koff(int row, int c) { return row * PITCH + kswz(row, c) * 16; }
-    __device__ static __forceinline__ int voff(int row, int c) { return row * PITCH + vswz(row, c) * 16; }
+    template <int MF> __device__ static __forceinline__ int voff(int row, int c) { return row * PITCH + vswz<MF>(row, c) * 16; }
 };
 // four rows x 16 columns of 16-bit elements, transposed: lane i of 16 gets column i of rows 0..3; the address of lane i is
 // that of row i / 4, columns 4 (i % 4) ..
@@ -46,10 +47,11 @@ __device__ __forceinline__ f32x16 mma32(float a, float b, f32x16 c) { return __b
 
 template <typename V> __device__ __forceinline__ V as(u32x4 v) { return __builtin_bit_cast(V, v); }
 // What is not there is read from here: a choice of addresses instead of a branch per load, behind which the compiler loses
-// count of the loads in flight and waits for all of them
+// count of the loads in flight and waits for all of them.  (Global pointers, said so: a generic one counts as an LDS access.)
 __device__ const u32x4 zero_piece = {0, 0, 0, 0};
+typedef const __attribute__((address_space(1))) u32x4* GlobalPiece;
 template <typename T> __device__ __forceinline__ u32x4 piece(const T* p, bool ok) {
-    return *(ok ? (const u32x4*)p : &zero_piece);
+    return *(ok ? (GlobalPiece)(uintptr_t)p : (GlobalPiece)(uintptr_t)&zero_piece);
 }
 
 // ---- one token per stream -------------------------------------------------------------------------------------------------
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
                 const bool here = (unsigned)page < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width, ok = here && key <= (unsigned)pos;
                 lost |= !here && key <= (unsigned)pos;
                 const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
-                const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::vswz(row, pc) * TL::PER;
+                const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::template vswz<16>(row, pc) * TL::PER;
                 kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
                 vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
             }
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
 #pragma unroll
                 for (int i = 0; i < DT; ++i) {
                     const int r = 4 * g + (l15 >> 2), c = 2 * i + ((l15 >> 1) & 1), o = (l15 & 1) * 8;
-                    s16x4 v[2] = {read_tr(vt_lds + TL::voff(r, c) + o), read_tr(vt_lds + TL::voff(r + 16, c) + o)};
+                    s16x4 v[2] = {read_tr(vt_lds + TL::template voff<16>(r, c) + o), read_tr(vt_lds + TL::template voff<16>(r + 16, c) + o)};
                     acc[i] = mma16(__builtin_bit_cast(typename Vec<T, 8>::type, v), pf, acc[i]);
                 }
             } else {
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
                 for (int i = 0; i < DT; ++i)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const float v = *(const float*)(vt_lds + TL::voff(4 * g + c, 4 * i + (l15 >> 2)) + (l15 & 3) * 4);
+                        const float v = *(const float*)(vt_lds + TL::template voff<16>(4 * g + c, 4 * i + (l15 >> 2)) + (l15 & 3) * 4);
                         acc[i] = mma16(v, sc[0][c], acc[i]);
                     }
             }
@@ -313,8 +315,19 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 }
 
 // ---- many rows per stream -------------------------------------------------------------------------------------------------
+// A block's waves have 32 rows each and share every tile of keys and values in LDS.  A tile's work is a vector part (softmax
+// of its scores) and a matrix part (its values, and the next tile's scores).  Waves w and w + 4 share a SIMD: the upper four
+// pass the tile's barrier between their vector and matrix parts, the lower four in front of both, so that the matrix cores
+// work for one while the other does its exponentials.  In the interval behind barrier k everybody reads V(k) and K(k+1) and
+// writes V(k+1) and K(k+2), requested an interval before: two buffers of each.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
+
+__device__ __forceinline__ float sum2(f16 a, f16 b, float x, float y, float l) { return l + x + y; }
+__device__ __forceinline__ float sum2(bfl a, bfl b, float, float, float l) {
+    typedef Vec<bfl, 2>::type B2;
+    return __builtin_amdgcn_fdot2_f32_bf16(B2{a, b}, B2{(bfl)1.f, (bfl)1.f}, l, false);   // two rounded weights in one instruction
+}
 
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_chunk(AttendArgs a) {
@@ -322,11 +335,12 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     typedef Tile<T, DP> TL;
     constexpr int LD = KT * TL::CPR / NT, TILE_BYTES = KT * TL::PITCH;
     typedef typename Vec<T, 8>::type V8;
-    extern __shared__ __attribute__((aligned(16))) char lds[];              // two buffers of a K and a V tile, flags
-    unsigned long long* flag = (unsigned long long*)(lds + 4 * TILE_BYTES); // [3]: rows of a V tile that are not finite
-    int* badf = (int*)(flag + 3);                                           // [3]: groups of 16 keys without a page
+    extern __shared__ __attribute__((aligned(16))) char lds[];              // K x 2, V x 2, flags
+    unsigned long long* flag = (unsigned long long*)(lds + 4 * TILE_BYTES); // [4]: rows of a V tile that held something not finite
+    int* badf = (int*)(flag + 4);                                           // [4]: groups of 16 keys without a page
     const PagedArgs& p = a.p;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, hf = lane >> 5;
+    const bool upper = wave >= 4;
     const int group = p.Hq / p.Hkv, Dh = p.Dh;
     const int kvh = blockIdx.x % p.Hkv, tile_id = blockIdx.x / p.Hkv;
     // ---- rows of no stream are 0
@@ -387,116 +401,119 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
     float m = -INFINITY, l = 0.f;
+    // ---- staging.  Page numbers are looked up a tile before they are used, each thread those of its own rows, and by vector
+    // loads: a scalar load would be waited for together with the LDS reads
     u32x4 kr[LD], vr[LD];
-    // Page numbers are looked up a tile before they are used, each thread those of its own rows, and by vector loads: a scalar
-    // load would be waited for together with the LDS reads.  entry[j]: what the table holds for the tile to be requested next
-    int entry[LD];
-    bool lost = false;                                                      // a row of mine in the tile requested last has no page
+    int e_k[LD], e_v[LD];                                                   // what the table holds for the next K and V tile
+    int lost = 0;                                                           // groups of the K tile requested last where a row of mine has no page
     const int page_mask = (1 << p.page_shift) - 1;
     const int* table = p.table + (int64_t)s * p.width;
     auto look = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < LD; ++j) entry[j] = table[min(((unsigned)t * KT + (j * NT + tid) / TL::CPR) >> p.page_shift, (unsigned)p.width - 1)];
+        for (int j = 0; j < LD; ++j) e_k[j] = table[min(((unsigned)t * KT + (j * NT + tid) / TL::CPR) >> p.page_shift, (unsigned)p.width - 1)];
     };
-    auto load = [&](int t) {
-        lost = false;
-        const T *kp[LD], *vp[LD];                                           // (all page numbers are used before a load is issued)
-        bool ok[LD];
+    auto place = [&](int t, int entry, int row, bool& here) {               // first element of a key's row; here: it has a page
+        const unsigned key = (unsigned)t * KT + row;
+        here = (unsigned)entry < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width;
+        return ((((int64_t)entry * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
+    };
+    // K(t) and V(t - 1); then the page numbers of K(t + 1).  (All page numbers are used before a load is issued.)
+    auto load = [&](int t, bool want_k, bool want_v) {
+        const T *kp[LD], *vp[LD];
+        bool k_ok[LD], v_ok[LD];
+        lost = 0;
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
-            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR;
-            const unsigned key = (unsigned)t * KT + row;
-            const bool here = (unsigned)entry[j] < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width;
-            ok[j] = here && key <= (unsigned)b_hi;
-            lost |= !here && key <= (unsigned)b_hi;
-            const int64_t base = ((((int64_t)entry[j] * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
-            kp[j] = (const T*)a.k_pages + base + TL::kswz(row, pc) * TL::PER;
-            vp[j] = (const T*)a.v_pages + base + TL::vswz(row, pc) * TL::PER;
+            const int i = j * NT + tid, row = i / TL::CPR, kc = TL::kswz(row, i % TL::CPR) * TL::PER, vc = TL::template vswz<32>(row, i % TL::CPR) * TL::PER;
+            bool here;
+            kp[j] = (const T*)a.k_pages + place(t, e_k[j], row, here) + kc;
+            const bool seen = want_k && (unsigned)t * KT + row <= (unsigned)b_hi;
+            k_ok[j] = seen && here && kc < Dh;
+            lost |= (seen && !here) << (row >> 4);
+            vp[j] = (const T*)a.v_pages + place(t - 1, e_v[j], row, here) + vc;
+            v_ok[j] = want_v && (unsigned)(t - 1) * KT + row <= (unsigned)b_hi && here && vc < Dh;
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            const int i = j * NT + tid, row = i / TL::CPR, pc = i % TL::CPR;
-            kr[j] = piece(kp[j], ok[j] && TL::kswz(row, pc) * TL::PER < Dh);
-            vr[j] = piece(vp[j], ok[j] && TL::vswz(row, pc) * TL::PER < Dh);
-        }
+        for (int j = 0; j < LD; ++j) { kr[j] = piece(kp[j], k_ok[j]); vr[j] = piece(vp[j], v_ok[j]); e_v[j] = e_k[j]; }
+        look(t + 1);
     };
-    if (tid < 3) { flag[tid] = 0; badf[tid] = 0; }
-    if (t_lo < t_hi) { look(t_lo); load(t_lo); look(t_lo + 1); }
-    __syncthreads();
-    for (int t = t_lo; t < t_hi; ++t) {
-        char* kt_lds = lds + ((t - t_lo) & 1) * 2 * TILE_BYTES;
-        char* vt_lds = kt_lds + TILE_BYTES;
-        const bool edge = b_lo - t * KT < KT - 1;                           // some row of the block does not see the whole tile
-        const int slot = (t - t_lo) % 3;                                    // flags are cleared two barriers before they are used again
+    auto store_k = [&](int t) {
+        char* to = lds + ((t - t_lo) & 1) * TILE_BYTES + tid * 16;
 #pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            *(u32x4*)(kt_lds + (j * NT + tid) * 16) = kr[j];
-            *(u32x4*)(vt_lds + (j * NT + tid) * 16) = vr[j];
-        }
-        if (edge) {
-            // a value that is not finite would reach rows that do not see it (0 x NaN): remember which keys hold one
+        for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = kr[j];
+        if (lost) atomicOr(badf + ((t - t_lo) & 3), lost);
+    };
+    auto store_v = [&](int t) {
+        if (b_lo - t * KT < KT - 1) {
+            // not every row of the block sees the whole tile: a value that is not finite would reach those that do not see it
+            // (0 x NaN).  It is stored as 0, and its key remembered
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
                 bool odd = false;
 #pragma unroll
                 for (int k = 0; k < TL::PER; ++k) {
-                    if constexpr (sizeof(T) == 4) odd |= !__builtin_isfinite(as<f32x4>(vr[j])[k]);
-                    else odd |= !__builtin_isfinite((float)as<V8>(vr[j])[k]);
-                }
-                if (odd) atomicOr(flag + slot, 1ull << ((j * NT + tid) / TL::CPR));
-            }
-        }
-        if (__any(lost)) {                                                  // (a page holds 16 keys or more: a group has one or none)
-#pragma unroll
-            for (int j = 0; j < LD; ++j) {
-                const unsigned row = (j * NT + tid) / TL::CPR, col = ((unsigned)t * KT + row) >> p.page_shift;
-                if (t * KT + row <= (unsigned)b_hi && (col >= (unsigned)p.width || (unsigned)table[col] >= (unsigned)p.pages)) atomicOr(badf + slot, 1 << (row >> 4));
-            }
-        }
-        __syncthreads();
-        if (tid == 0) { const int next = slot == 0 ? 2 : slot - 1; flag[next] = 0; badf[next] = 0; }
-        if (t + 1 < t_hi) { load(t + 1); look(t + 2); }
-        const unsigned long long keys = edge ? flag[slot] : 0;
-        if (keys) {
-            for (int k = 0; k < KT; ++k) {
-                if (!(keys >> k & 1) || pos - t * KT < k) continue;
-#pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const int d = i * 32 + 8 * (c >> 2) + 4 * hf + (c & 3);
-                        const float v = (float)*(const T*)(vt_lds + TL::voff(k, d / TL::PER) + d % TL::PER * (int)sizeof(T));
-                        if (!__builtin_isfinite(v)) acc[i][c] += v;         // whatever its weight, the sum is not finite
+                    if constexpr (sizeof(T) == 4) {
+                        f32x4 v = as<f32x4>(vr[j]);
+                        if (!__builtin_isfinite(v[k])) { odd = true; v[k] = 0.f; vr[j] = __builtin_bit_cast(u32x4, v); }
+                    } else {
+                        V8 v = as<V8>(vr[j]);
+                        if (!__builtin_isfinite((float)v[k])) { odd = true; v[k] = (T)0.f; vr[j] = __builtin_bit_cast(u32x4, v); }
                     }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < LD; ++j) {
-                char* at = vt_lds + (j * NT + tid) * 16;
-#pragma unroll
-                for (int k = 0; k < TL::PER; ++k)
-                    if (!__builtin_isfinite((float)((T*)at)[k])) ((T*)at)[k] = (T)0.f;
-            }
-            __syncthreads();
-        }
-        if (t * KT <= w_hi) {
-            const int bad = badf[slot];
-            f32x16 sc[NK];
-#pragma unroll
-            for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-                for (int c = 0; c < 16; ++c) sc[kt][c] = 0.f;
-#pragma unroll
-            for (int i = 0; i < TL::CPR / 2; ++i)
-#pragma unroll
-                for (int kt = 0; kt < NK; ++kt) {
-                    const u32x4 kf = *(const u32x4*)(kt_lds + TL::koff(kt * 32 + l31, 2 * i + hf));
-                    if constexpr (sizeof(T) == 2) sc[kt] = mma32(as<V8>(kf), as<V8>(qf[i]), sc[kt]);
-                    else
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) sc[kt] = mma32(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
                 }
+                if (odd) atomicOr(flag + ((t - t_lo) & 3), 1ull << ((j * NT + tid) / TL::CPR));
+            }
+        }
+        char* to = lds + (2 + ((t - t_lo) & 1)) * TILE_BYTES + tid * 16;
+#pragma unroll
+        for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = vr[j];
+    };
+    f32x16 sc[NK];
+    auto scores = [&](int t) {                                              // lane = (row l31, keys 8 b + 4 hf + 0..3 of each 32)
+        const char* k_lds = lds + ((t - t_lo) & 1) * TILE_BYTES;
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) sc[kt][c] = 0.f;
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 2; ++i)
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt) {
+                const u32x4 kf = *(const u32x4*)(k_lds + TL::koff(kt * 32 + l31, 2 * i + hf));
+                if constexpr (sizeof(T) == 2) sc[kt] = mma32(as<V8>(kf), as<V8>(qf[i]), sc[kt]);
+                else
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sc[kt] = mma32(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
+            }
+        if constexpr (sizeof(T) == 2) {
+            // the reads of four products are in flight ahead of the matrix instructions (0x100: LDS read, 0x008: MFMA)
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < NK * TL::CPR / 2 - 4; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        }
+    };
+    if (tid < 4) { flag[tid] = 0; badf[tid] = 0; }
+    __syncthreads();
+    if (t_lo < t_hi) {
+        look(t_lo);
+        load(t_lo, true, false);
+        store_k(t_lo);
+        load(t_lo + 1, t_lo + 1 < t_hi, true);
+        store_k(t_lo + 1);
+        store_v(t_lo);
+    }
+    __syncthreads();
+    if (t_lo < t_hi && t_lo * KT <= w_hi) scores(t_lo);
+    for (int t = t_lo; t < t_hi; ++t) {
+        if (!upper) __syncthreads();
+        const bool more = t + 1 < t_hi, mine = t * KT <= w_hi;
+        if (more) load(t + 2, t + 2 < t_hi, true);
+        if (tid == 0) { flag[(t - t_lo + 2) & 3] = 0; badf[(t - t_lo + 3) & 3] = 0; }       // last read an interval ago, next set an interval on
+        V8 pf[sizeof(T) == 2 ? KT / 16 : 1];
+        f32x16 pw[sizeof(T) == 4 ? NK : 1];
+        if (mine) {
+            const int bad = badf[(t - t_lo) & 3], left = pos - t * KT;      // keys of the tile the row sees: 0 .. left
             if (bad) {                                                      // scores of keys without a page: not a number
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
@@ -508,8 +525,7 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-                    for (int c = 0; c < 16; ++c)
-                        sc[kt][c] = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= pos - t * KT ? sc[kt][c] : -INFINITY;
+                    for (int c = 0; c < 16; ++c) sc[kt][c] = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= left ? sc[kt][c] : -INFINITY;
             }
             float mt = sc[0][0];
 #pragma unroll
@@ -530,20 +546,55 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
             for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-                for (int c = 0; c < 16; ++c) { sc[kt][c] = exp2_hw(fmaf(sc[kt][c], a.scale_log2e, -ms)); l += sc[kt][c]; }
+                for (int c = 0; c < 16; c += 2) {
+                    const float x = exp2_hw(fmaf(sc[kt][c], a.scale_log2e, -ms)), y = exp2_hw(fmaf(sc[kt][c + 1], a.scale_log2e, -ms));
+                    if constexpr (sizeof(T) == 2) {                         // weights rounded to the tensors' type for the matrix instruction
+                        V8& v = pf[kt * 2 + (c >> 3)];
+                        v[c & 7] = (T)x; v[(c & 7) + 1] = (T)y;
+                        l = sum2(v[c & 7], v[(c & 7) + 1], x, y, l);
+                    } else { pw[kt][c] = x; pw[kt][c + 1] = y; l += x + y; }
+                }
+        }
+        if (upper) __syncthreads();                                         // (the same barrier: every wave passes one per tile)
+        __builtin_amdgcn_s_setprio(1);
+        if (more && (t + 1) * KT <= w_hi) scores(t + 1);
+        if (mine) {
+            const char* v_lds = lds + (2 + ((t - t_lo) & 1)) * TILE_BYTES;
+            if (b_lo - t * KT < KT - 1) {
+                const unsigned long long keys = flag[(t - t_lo) & 3];
+                if (keys) {
+#pragma nounroll
+                    for (int k = 0; k < KT; ++k) {                          // whatever its weight, what is not finite decides the sum
+                        if (!(keys >> k & 1) || pos - t * KT < k) continue;
+                        bool here;
+                        const int col = min((t * KT + k) >> p.page_shift, p.width - 1);
+                        const T* v = (const T*)a.v_pages + place(t, table[col], k, here) + 4 * hf;
+                        if (!here) continue;
+#pragma unroll
+                        for (int i = 0; i < DT; ++i)
+#pragma unroll
+                            for (int c = 0; c < 16; c += 4) {
+                                typedef typename Vec<T, 4>::type V4;
+                                const V4 x = i * 32 + 2 * c + 4 * hf < Dh ? *(const V4*)(v + i * 32 + 2 * c) : V4{};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[i][c + e] += __builtin_isfinite((float)x[e]) ? 0.f : (float)x[e];
+                            }
+                    }
+                }
+            }
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int k16 = 0; k16 < KT / 16; ++k16) {
-                    V8 pf;                                                  // weights rounded to the tensors' type for the matrix instruction
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) pf[c] = (T)sc[k16 >> 1][(k16 & 1) * 8 + c];
+                for (int k16 = 0; k16 < KT / 16; ++k16)
 #pragma unroll
                     for (int i = 0; i < DT; ++i) {
                         const int row = k16 * 16 + 4 * hf + ((lane & 15) >> 2), c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), o = (lane & 1) * 8;
-                        s16x4 v[2] = {read_tr(vt_lds + TL::voff(row, c) + o), read_tr(vt_lds + TL::voff(row + 8, c) + o)};
-                        acc[i] = mma32(__builtin_bit_cast(V8, v), pf, acc[i]);
+                        s16x4 v[2] = {read_tr(v_lds + TL::template voff<32>(row, c) + o), read_tr(v_lds + TL::template voff<32>(row + 8, c) + o)};
+                        acc[i] = mma32(__builtin_bit_cast(V8, v), pf[k16], acc[i]);
                     }
-                }
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+                for (int i = 0; i < KT / 16 * DT - 4; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
             } else {
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
@@ -552,10 +603,12 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
                         const int row = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3);
 #pragma unroll
                         for (int i = 0; i < DT; ++i)
-                            acc[i] = mma32(*(const float*)(vt_lds + TL::voff(row, 8 * i + (l31 >> 2)) + (l31 & 3) * 4), sc[kt][c], acc[i]);
+                            acc[i] = mma32(*(const float*)(v_lds + TL::template voff<32>(row, 8 * i + (l31 >> 2)) + (l31 & 3) * 4), pw[kt][c], acc[i]);
                     }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
+        if (more) { store_k(t + 2); store_v(t + 1); }
     }
     l += __shfl_xor(l, 32);
     if (r >= n_rows) return;
@@ -641,7 +694,7 @@ template <typename T, int DP> void run_one(AttendArgs a, hipStream_t s) {
     if (a.splits) attend_join<T, DP><<<(unsigned)segs, DP, 0, s>>>(a, keys);
 }
 template <typename T, int DP, int NW> void run_chunk_nw(AttendArgs a, hipStream_t s) {
-    constexpr int bytes = 4 * chunk_kt<T>() * DP * (int)sizeof(T) + 64;
+    constexpr int bytes = 4 * chunk_kt<T>() * DP * (int)sizeof(T) + 48;
     static bool set[64];                                        // per device: more LDS than a kernel gets by default
     int dev = 0;
     (void)hipGetDevice(&dev);
