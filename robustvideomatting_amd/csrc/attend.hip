@@ -323,6 +323,11 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
 
+// the larger of a lane's value and that of the lane 32 away
+__device__ __forceinline__ float max_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
 __device__ __forceinline__ float sum2(f16 a, f16 b, float x, float y, float l) { return l + x + y; }
 __device__ __forceinline__ float sum2(bfl a, bfl b, float, float, float l) {
     typedef Vec<bfl, 2>::type B2;
@@ -401,48 +406,60 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
     float m = -INFINITY, l = 0.f;
-    // ---- staging.  Page numbers are looked up a tile before they are used, each thread those of its own rows, and by vector
-    // loads: a scalar load would be waited for together with the LDS reads
+    // ---- staging.  The 64 pieces that a wave requests at once lie in one group of 16 keys, hence in one page: their place is
+    // scalar arithmetic, plus an offset of the lane's own that never changes.  Page numbers are looked up a tile before they are
+    // used, by vector loads: a scalar load would be waited for together with the LDS reads
     u32x4 kr[LD], vr[LD];
     int e_k[LD], e_v[LD];                                                   // what the table holds for the next K and V tile
-    int lost = 0;                                                           // groups of the K tile requested last where a row of mine has no page
+    int grp[LD];                                                            // first key of the group
+    unsigned k_off[LD], v_off[LD];
+    bool k_in[LD];
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+        const int i = j * NT + tid, row = i / TL::CPR, kc = TL::kswz(row, i % TL::CPR) * TL::PER, vc = TL::template vswz<32>(row, i % TL::CPR) * TL::PER;
+        grp[j] = __builtin_amdgcn_readfirstlane(row & ~15);
+        k_in[j] = kc < Dh;
+        k_off[j] = ((row & 15) * Dh + (k_in[j] ? kc : 0)) * (unsigned)sizeof(T);
+        v_off[j] = ((row & 15) * Dh + (vc < Dh ? vc : 0)) * (unsigned)sizeof(T);
+    }
+    int lost = 0;                                                           // groups of the K tile requested last that have no page
     const int page_mask = (1 << p.page_shift) - 1;
     const int* table = p.table + (int64_t)s * p.width;
     auto look = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < LD; ++j) e_k[j] = table[min(((unsigned)t * KT + (j * NT + tid) / TL::CPR) >> p.page_shift, (unsigned)p.width - 1)];
+        for (int j = 0; j < LD; ++j) e_k[j] = table[min(((unsigned)t * KT + grp[j] + (lane & 15)) >> p.page_shift, (unsigned)p.width - 1)];
     };
-    auto place = [&](int t, int entry, int row, bool& here) {               // first element of a key's row; here: it has a page
-        const unsigned key = (unsigned)t * KT + row;
+    // first byte of the group's keys in a pool; a group without a page reads page 0 (and is flagged)
+    auto place = [&](int t, int entry, int first, bool& here) {
+        const unsigned key = (unsigned)t * KT + first;
         here = (unsigned)entry < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width;
-        return ((((int64_t)entry * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
+        return ((((int64_t)(here ? entry : 0) * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh * (int)sizeof(T);
     };
-    // K(t) and V(t - 1); then the page numbers of K(t + 1).  (All page numbers are used before a load is issued.)
-    auto load = [&](int t, bool want_k, bool want_v) {
-        const T *kp[LD], *vp[LD];
-        bool k_ok[LD], v_ok[LD];
+    // K(t) and V(t - 1); then the page numbers of K(t + 1).  Keys behind the last one that a row sees are whatever their page
+    // holds (in bounds: a page ends behind its last slot): their scores are masked, and store_v lets nothing through but numbers
+    auto load = [&](int t) {
+        const char *kp[LD], *vp[LD];
         lost = 0;
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
-            const int i = j * NT + tid, row = i / TL::CPR, kc = TL::kswz(row, i % TL::CPR) * TL::PER, vc = TL::template vswz<32>(row, i % TL::CPR) * TL::PER;
             bool here;
-            kp[j] = (const T*)a.k_pages + place(t, e_k[j], row, here) + kc;
-            const bool seen = want_k && (unsigned)t * KT + row <= (unsigned)b_hi;
-            k_ok[j] = seen && here && kc < Dh;
-            lost |= (seen && !here) << (row >> 4);
-            vp[j] = (const T*)a.v_pages + place(t - 1, e_v[j], row, here) + vc;
-            v_ok[j] = want_v && (unsigned)(t - 1) * KT + row <= (unsigned)b_hi && here && vc < Dh;
+            kp[j] = (const char*)a.k_pages + place(t, __builtin_amdgcn_readfirstlane(e_k[j]), grp[j], here);
+            lost |= (!here && (unsigned)t * KT + grp[j] <= (unsigned)b_hi) << (grp[j] >> 4);
+            vp[j] = (const char*)a.v_pages + place(t - 1, __builtin_amdgcn_readfirstlane(e_v[j]), grp[j], here);
+            e_v[j] = e_k[j];
         }
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < LD; ++j) { kr[j] = piece(kp[j], k_ok[j]); vr[j] = piece(vp[j], v_ok[j]); e_v[j] = e_k[j]; }
+        for (int j = 0; j < LD; ++j) { kr[j] = *(const u32x4*)(kp[j] + k_off[j]); vr[j] = *(const u32x4*)(vp[j] + v_off[j]); }
         look(t + 1);
     };
     auto store_k = [&](int t) {
+        if (Dh < DP)                                                        // dims past the head: zeros, as in Q
+#pragma unroll
+            for (int j = 0; j < LD; ++j) kr[j] = k_in[j] ? kr[j] : u32x4{0, 0, 0, 0};
         char* to = lds + ((t - t_lo) & 1) * TILE_BYTES + tid * 16;
 #pragma unroll
         for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = kr[j];
-        if (lost) atomicOr(badf + ((t - t_lo) & 3), lost);
+        if (lost && lane == 0) atomicOr(badf + ((t - t_lo) & 3), lost);
     };
     auto store_v = [&](int t) {
         if (b_lo - t * KT < KT - 1) {
@@ -468,9 +485,11 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
         for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = vr[j];
     };
+    int bad = 0;                                                            // groups of the tile of sc that have no page
     f32x16 sc[NK];
     auto scores = [&](int t) {                                              // lane = (row l31, keys 8 b + 4 hf + 0..3 of each 32)
         const char* k_lds = lds + ((t - t_lo) & 1) * TILE_BYTES;
+        bad = badf[(t - t_lo) & 3];
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
@@ -497,9 +516,11 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     __syncthreads();
     if (t_lo < t_hi) {
         look(t_lo);
-        load(t_lo, true, false);
+#pragma unroll
+        for (int j = 0; j < LD; ++j) e_v[j] = 0;
+        load(t_lo);
         store_k(t_lo);
-        load(t_lo + 1, t_lo + 1 < t_hi, true);
+        load(t_lo + 1);
         store_k(t_lo + 1);
         store_v(t_lo);
     }
@@ -508,13 +529,13 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     for (int t = t_lo; t < t_hi; ++t) {
         if (!upper) __syncthreads();
         const bool more = t + 1 < t_hi, mine = t * KT <= w_hi;
-        if (more) load(t + 2, t + 2 < t_hi, true);
+        load(t + 2);                                                        // (past the end too: in bounds, never used, and no branch around loads in flight)
         if (tid == 0) { flag[(t - t_lo + 2) & 3] = 0; badf[(t - t_lo + 3) & 3] = 0; }       // last read an interval ago, next set an interval on
         V8 pf[sizeof(T) == 2 ? KT / 16 : 1];
         f32x16 pw[sizeof(T) == 4 ? NK : 1];
         if (mine) {
-            const int bad = badf[(t - t_lo) & 3], left = pos - t * KT;      // keys of the tile the row sees: 0 .. left
-            if (bad) {                                                      // scores of keys without a page: not a number
+            const int left = pos - t * KT;                                  // keys of the tile the row sees: 0 .. left
+            if (__builtin_amdgcn_readfirstlane(bad)) {                                                      // scores of keys without a page: not a number
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
@@ -532,7 +553,7 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
             for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                 for (int c = 0; c < 16; ++c) mt = fmaxf(mt, sc[kt][c]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32)) * a.scale_log2e;
+            mt = max_of_halves(mt) * a.scale_log2e;
             if (__any(mt > m + LAZY)) {
                 const float mn = fmaxf(m, mt), al = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
                 m = mn;
@@ -568,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
                         if (!(keys >> k & 1) || pos - t * KT < k) continue;
                         bool here;
                         const int col = min((t * KT + k) >> p.page_shift, p.width - 1);
-                        const T* v = (const T*)a.v_pages + place(t, table[col], k, here) + 4 * hf;
+                        const T* v = (const T*)((const char*)a.v_pages + place(t, table[col], k, here)) + 4 * hf;
                         if (!here) continue;
 #pragma unroll
                         for (int i = 0; i < DT; ++i)
@@ -608,7 +629,8 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        if (more) { store_k(t + 2); store_v(t + 1); }
+        store_k(t + 2);
+        store_v(t + 1);
     }
     l += __shfl_xor(l, 32);
     if (r >= n_rows) return;
