@@ -7,6 +7,7 @@
 //   attend_one    one new token per stream: the rows of a tile are the query heads that share a key head (16 x 16 tiles)
 //   attend_chunk  many rows per stream: (token, head of the group) pairs share every key they read (32 x 32 tiles)
 #include "temporal.hpp"
+#include <type_traits>
 
 namespace {
 
@@ -284,12 +285,16 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
     }
 }
 
-// Adds the pieces of the segments that no block of attend_one had whole, in the order of the keys.  One block per segment.
+// Adds the pieces of the segments that no block of attend_one had whole, in the order of the keys.  One block per segment and
+// query head; the pieces' factors first, so that their rows are requested side by side.
 template <typename T, int DP>
 __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
+    __shared__ float factor[ONE_GRID];
     const PagedArgs& p = a.p;
     const int group = p.Hq / p.Hkv, rts = (group + 15) / 16, segs = p.Hkv * rts, lane = threadIdx.x & 63;
-    const int s = blockIdx.x / segs, seg = blockIdx.x % segs, d = threadIdx.x;
+    const int s = blockIdx.x / segs, seg = blockIdx.x % segs, d = threadIdx.x, r = blockIdx.y;
+    const int kvh = seg / rts, h0 = kvh * group + (seg - kvh * rts) * 16;
+    if (r >= kvh * group + group - h0) return;
     const int n = Units::of_stream(p, s, keys);
     if (!n) return;
     Units U;
@@ -297,29 +302,32 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
     int64_t before = 0;
     for (int b = 0; b < s; b += 64) before += b + lane < s ? Units::of_stream(p, b + lane, keys) : 0;
     for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
-    const int64_t first = before * segs + (int64_t)seg * n, b0 = first / U.per, b1 = (first + n - 1) / U.per;
+    const int64_t first = before * segs + (int64_t)seg * n;
+    const int b0 = (int)(first / U.per), b1 = (int)((first + n - 1) / U.per);
     if (b0 == b1) return;
-    const int kvh = seg / rts, h0 = kvh * group + (seg - kvh * rts) * 16, rows = min(16, kvh * group + group - h0);
-    for (int r = 0; r < rows; ++r) {
-        float M = -INFINITY, L = 0.f, acc = 0.f;
-        for (int64_t b = b0; b <= b1; ++b) {
-            const float* o = a.part + (b * 2 + (b == b0)) * piece_floats(DP);
-            const float m = o[ONE_ROWS * DP + r], l = o[ONE_ROWS * (DP + 1) + r], mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
-            const float ea = exp2_hw(M - ms), eb = exp2_hw(m - ms);
-            acc = acc * ea + o[r * DP + d] * eb;
-            L = L * ea + l * eb;
-            M = mn;
-        }
-        if (d < p.Dh) ((T*)a.out)[((int64_t)s * p.Hq + h0 + r) * p.Dh + d] = (T)(acc / L);
+    auto piece_of = [&](int b) { return a.part + ((int64_t)b * 2 + (b == b0)) * piece_floats(DP); };
+    float M = -INFINITY, L = 0.f;
+    for (int b = b0 + lane; b <= b1; b += 64) M = fmaxf(M, piece_of(b)[ONE_ROWS * DP + r]);
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float MS = M == -INFINITY ? 0.f : M;
+    for (int b = b0 + lane; b <= b1; b += 64) {
+        const float* o = piece_of(b);
+        const float f = exp2_hw(o[ONE_ROWS * DP + r] - MS);
+        if (d < 64) factor[b - b0] = f;
+        L += o[ONE_ROWS * (DP + 1) + r] * f;
     }
+    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
+    __syncthreads();
+    float acc = 0.f;
+#pragma unroll 8
+    for (int b = b0; b <= b1; ++b) acc = fmaf(piece_of(b)[r * DP + d], factor[b - b0], acc);
+    if (d < p.Dh) ((T*)a.out)[((int64_t)s * p.Hq + h0 + r) * p.Dh + d] = (T)(acc / L);
 }
 
 // ---- many rows per stream -------------------------------------------------------------------------------------------------
-// A block's waves have 32 rows each and share every tile of keys and values in LDS.  A tile's work is a vector part (softmax
-// of its scores) and a matrix part (its values, and the next tile's scores).  Waves w and w + 4 share a SIMD: the upper four
-// pass the tile's barrier between their vector and matrix parts, the lower four in front of both, so that the matrix cores
-// work for one while the other does its exponentials.  In the interval behind barrier k everybody reads V(k) and K(k+1) and
-// writes V(k+1) and K(k+2), requested an interval before: two buffers of each.
+// A block's four waves have 32 rows each and share every tile of keys and values in LDS: two buffers, one barrier per tile, the
+// next tile requested at the start of a tile and stored at its end.  Inside a wave the exponentials of 16 keys run under the
+// matrix instructions of the 16 before them.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
 
@@ -334,9 +342,11 @@ __device__ __forceinline__ float sum2(bfl a, bfl b, float, float, float l) {
     return __builtin_amdgcn_fdot2_f32_bf16(B2{a, b}, B2{(bfl)1.f, (bfl)1.f}, l, false);   // two rounded weights in one instruction
 }
 
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_chunk(AttendArgs a) {
-    constexpr int KT = chunk_kt<T>(), NK = KT / 32, R = 32 * NW, NT = 64 * NW, DT = DP / 32;
+constexpr int CHUNK_WAVES = 4, CHUNK_ROWS = 32 * CHUNK_WAVES;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2) void attend_chunk(AttendArgs a) {
+    constexpr int KT = chunk_kt<T>(), NK = KT / 32, R = CHUNK_ROWS, NT = 64 * CHUNK_WAVES, DT = DP / 32;
     typedef Tile<T, DP> TL;
     constexpr int LD = KT * TL::CPR / NT, TILE_BYTES = KT * TL::PITCH;
     typedef typename Vec<T, 8>::type V8;
@@ -345,7 +355,6 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     int* badf = (int*)(flag + 4);                                           // [4]: groups of 16 keys without a page
     const PagedArgs& p = a.p;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, hf = lane >> 5;
-    const bool upper = wave >= 4;
     const int group = p.Hq / p.Hkv, Dh = p.Dh;
     const int kvh = blockIdx.x % p.Hkv, tile_id = blockIdx.x / p.Hkv;
     // ---- rows of no stream are 0
@@ -387,8 +396,6 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     auto at = [&](int token) { return (int)min((int64_t)INT32_MAX, max((int64_t)-1, (int64_t)past + token)); };
     const int r = row0 + wave * 32 + l31, rr = min(r, n_rows - 1), tok = rr / group, h = kvh * group + rr - tok * group;
     const int pos = at(tok);                                                // this lane's row sees keys up to here
-    const int wr_lo = min(row0 + wave * 32, n_rows - 1), wr_hi = min(row0 + wave * 32 + 31, n_rows - 1);
-    const int w_lo = at(wr_lo / group), w_hi = at(wr_hi / group);           // least and largest of the wave
     const int b_lo = at(row0 / group), b_hi = at((min(row0 + R, n_rows) - 1) / group);
     int t_lo = 0, t_hi = b_hi < 0 ? 0 : b_hi / KT + 1;
     if (a.splits > 1) {
@@ -410,52 +417,53 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
     // scalar arithmetic, plus an offset of the lane's own that never changes.  Page numbers are looked up a tile before they are
     // used, by vector loads: a scalar load would be waited for together with the LDS reads
     u32x4 kr[LD], vr[LD];
-    int e_k[LD], e_v[LD];                                                   // what the table holds for the next K and V tile
+    int entry[LD];                                                          // what the table holds for the next tile
     int grp[LD];                                                            // first key of the group
     unsigned k_off[LD], v_off[LD];
-    bool k_in[LD];
+    const unsigned row_bytes = Dh * (unsigned)sizeof(T), page_mask = (1u << p.page_shift) - 1, table_keys = (unsigned)p.width << p.page_shift;
+    const unsigned page_bytes = (p.Hkv << p.page_shift) * row_bytes;
+    const char *k_pool = (const char*)a.k_pages + ((int64_t)kvh << p.page_shift) * row_bytes, *v_pool = (const char*)a.v_pages + ((int64_t)kvh << p.page_shift) * row_bytes;
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-        const int i = j * NT + tid, row = i / TL::CPR, kc = TL::kswz(row, i % TL::CPR) * TL::PER, vc = TL::template vswz<32>(row, i % TL::CPR) * TL::PER;
-        grp[j] = __builtin_amdgcn_readfirstlane(row & ~15);
-        k_in[j] = kc < Dh;
-        k_off[j] = ((row & 15) * Dh + (k_in[j] ? kc : 0)) * (unsigned)sizeof(T);
-        v_off[j] = ((row & 15) * Dh + (vc < Dh ? vc : 0)) * (unsigned)sizeof(T);
+        const int i = j * NT + tid, rw = i / TL::CPR, kc = TL::kswz(rw, i % TL::CPR) * TL::PER, vc = TL::template vswz<32>(rw, i % TL::CPR) * TL::PER;
+        grp[j] = __builtin_amdgcn_readfirstlane(rw & ~15);
+        k_off[j] = (rw & 15) * row_bytes + (kc < Dh ? kc : 0) * (unsigned)sizeof(T);
+        v_off[j] = (rw & 15) * row_bytes + (vc < Dh ? vc : 0) * (unsigned)sizeof(T);
     }
-    int lost = 0;                                                           // groups of the K tile requested last that have no page
-    const int page_mask = (1 << p.page_shift) - 1;
+    int lost = 0;                                                           // groups of the tile requested last that have no page
     const int* table = p.table + (int64_t)s * p.width;
     auto look = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < LD; ++j) e_k[j] = table[min(((unsigned)t * KT + grp[j] + (lane & 15)) >> p.page_shift, (unsigned)p.width - 1)];
+        for (int j = 0; j < LD; ++j) entry[j] = table[min(((unsigned)t * KT + grp[j] + (lane & 15)) >> p.page_shift, (unsigned)p.width - 1)];
     };
-    // first byte of the group's keys in a pool; a group without a page reads page 0 (and is flagged)
-    auto place = [&](int t, int entry, int first, bool& here) {
-        const unsigned key = (unsigned)t * KT + first;
-        here = (unsigned)entry < (unsigned)p.pages && key >> p.page_shift < (unsigned)p.width;
-        return ((((int64_t)(here ? entry : 0) * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh * (int)sizeof(T);
+    // bytes into a pool of the group of keys from `key` on; one without a page reads page 0 (and is flagged)
+    auto place = [&](unsigned key, int page, bool& here) -> int64_t {
+        here = (unsigned)page < (unsigned)p.pages && key < table_keys;
+        return (int64_t)((uint64_t)(unsigned)(here ? page : 0) * page_bytes) + (key & page_mask) * row_bytes;
     };
-    // K(t) and V(t - 1); then the page numbers of K(t + 1).  Keys behind the last one that a row sees are whatever their page
-    // holds (in bounds: a page ends behind its last slot): their scores are masked, and store_v lets nothing through but numbers
+    // tile t; then the page numbers of tile t + 1.  Past the last tile too: in bounds, never used, and no branch around
+    // loads in flight.  Keys behind the last one that a row sees are whatever their page holds (in bounds: a page ends behind
+    // its last slot): their scores are masked, and store_v lets nothing through but numbers
     auto load = [&](int t) {
-        const char *kp[LD], *vp[LD];
         lost = 0;
 #pragma unroll
         for (int j = 0; j < LD; ++j) {
             bool here;
-            kp[j] = (const char*)a.k_pages + place(t, __builtin_amdgcn_readfirstlane(e_k[j]), grp[j], here);
-            lost |= (!here && (unsigned)t * KT + grp[j] <= (unsigned)b_hi) << (grp[j] >> 4);
-            vp[j] = (const char*)a.v_pages + place(t - 1, __builtin_amdgcn_readfirstlane(e_v[j]), grp[j], here);
-            e_v[j] = e_k[j];
+            const unsigned key = (unsigned)t * KT + grp[j];
+            const int64_t where = place(key, __builtin_amdgcn_readfirstlane(entry[j]), here);
+            lost |= (!here && key <= (unsigned)b_hi) << (grp[j] >> 4);
+            kr[j] = *(const u32x4*)(k_pool + where + k_off[j]);
+            vr[j] = *(const u32x4*)(v_pool + where + v_off[j]);
         }
-#pragma unroll
-        for (int j = 0; j < LD; ++j) { kr[j] = *(const u32x4*)(kp[j] + k_off[j]); vr[j] = *(const u32x4*)(vp[j] + v_off[j]); }
         look(t + 1);
     };
     auto store_k = [&](int t) {
         if (Dh < DP)                                                        // dims past the head: zeros, as in Q
 #pragma unroll
-            for (int j = 0; j < LD; ++j) kr[j] = k_in[j] ? kr[j] : u32x4{0, 0, 0, 0};
+            for (int j = 0; j < LD; ++j) {
+                const int i = j * NT + tid;
+                if (TL::kswz(i / TL::CPR, i % TL::CPR) * TL::PER >= Dh) kr[j] = u32x4{0, 0, 0, 0};
+            }
         char* to = lds + ((t - t_lo) & 1) * TILE_BYTES + tid * 16;
 #pragma unroll
         for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = kr[j];
@@ -485,11 +493,13 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
         for (int j = 0; j < LD; ++j) *(u32x4*)(to + j * NT * 16) = vr[j];
     };
-    int bad = 0;                                                            // groups of the tile of sc that have no page
-    f32x16 sc[NK];
-    auto scores = [&](int t) {                                              // lane = (row l31, keys 8 b + 4 hf + 0..3 of each 32)
-        const char* k_lds = lds + ((t - t_lo) & 1) * TILE_BYTES;
-        bad = badf[(t - t_lo) & 3];
+    auto tile = [&](int t, auto plain) __attribute__((always_inline)) {
+        constexpr bool PLAIN = decltype(plain)::value;                      // every row of the block sees the whole tile, every key has a page
+        const char *k_lds = lds + ((t - t_lo) & 1) * TILE_BYTES, *v_lds = k_lds + 2 * TILE_BYTES;
+        load(t + 1);
+        if (tid == 0) { flag[(t - t_lo + 2) & 3] = 0; badf[(t - t_lo + 2) & 3] = 0; }       // last read two barriers ago, next set behind the next
+        // ---- scores: lane = (row l31, keys 8 b + 4 hf + 0..3 of each 32)
+        f32x16 sc[NK];
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
@@ -504,134 +514,110 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 || NW < 4) ? 1 : 2) void attend_
 #pragma unroll
                     for (int c = 0; c < 4; ++c) sc[kt] = mma32(as<f32x4>(kf)[c], as<f32x4>(qf[i])[c], sc[kt]);
             }
-        if constexpr (sizeof(T) == 2) {
-            // the reads of four products are in flight ahead of the matrix instructions (0x100: LDS read, 0x008: MFMA)
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-            for (int i = 0; i < NK * TL::CPR / 2 - 4; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
-            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        }
-    };
-    if (tid < 4) { flag[tid] = 0; badf[tid] = 0; }
-    __syncthreads();
-    if (t_lo < t_hi) {
-        look(t_lo);
-#pragma unroll
-        for (int j = 0; j < LD; ++j) e_v[j] = 0;
-        load(t_lo);
-        store_k(t_lo);
-        load(t_lo + 1);
-        store_k(t_lo + 1);
-        store_v(t_lo);
-    }
-    __syncthreads();
-    if (t_lo < t_hi && t_lo * KT <= w_hi) scores(t_lo);
-    for (int t = t_lo; t < t_hi; ++t) {
-        if (!upper) __syncthreads();
-        const bool more = t + 1 < t_hi, mine = t * KT <= w_hi;
-        load(t + 2);                                                        // (past the end too: in bounds, never used, and no branch around loads in flight)
-        if (tid == 0) { flag[(t - t_lo + 2) & 3] = 0; badf[(t - t_lo + 3) & 3] = 0; }       // last read an interval ago, next set an interval on
-        V8 pf[sizeof(T) == 2 ? KT / 16 : 1];
-        f32x16 pw[sizeof(T) == 4 ? NK : 1];
-        if (mine) {
-            const int left = pos - t * KT;                                  // keys of the tile the row sees: 0 .. left
-            if (__builtin_amdgcn_readfirstlane(bad)) {                                                      // scores of keys without a page: not a number
+        if (!PLAIN) {
+            const int bad = __builtin_amdgcn_readfirstlane(badf[(t - t_lo) & 3]);
+            if (bad) {                                                      // scores of keys without a page: not a number
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
                         if (bad >> (kt * 2 + (c >> 3)) & 1) sc[kt][c] = NAN;
             }
-            if (w_lo - t * KT < KT - 1) {
-#pragma unroll
-                for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) sc[kt][c] = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3) <= left ? sc[kt][c] : -INFINITY;
-            }
-            float mt = sc[0][0];
+            const int left = pos - t * KT - 4 * hf;                         // keys of the tile the row sees, from this lane's first on: 0 .. left
 #pragma unroll
             for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-                for (int c = 0; c < 16; ++c) mt = fmaxf(mt, sc[kt][c]);
-            mt = max_of_halves(mt) * a.scale_log2e;
-            if (__any(mt > m + LAZY)) {
-                const float mn = fmaxf(m, mt), al = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) acc[i][c] *= al;
-            }
-            const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-                for (int c = 0; c < 16; c += 2) {
-                    const float x = exp2_hw(fmaf(sc[kt][c], a.scale_log2e, -ms)), y = exp2_hw(fmaf(sc[kt][c + 1], a.scale_log2e, -ms));
-                    if constexpr (sizeof(T) == 2) {                         // weights rounded to the tensors' type for the matrix instruction
-                        V8& v = pf[kt * 2 + (c >> 3)];
-                        v[c & 7] = (T)x; v[(c & 7) + 1] = (T)y;
-                        l = sum2(v[c & 7], v[(c & 7) + 1], x, y, l);
-                    } else { pw[kt][c] = x; pw[kt][c + 1] = y; l += x + y; }
-                }
+                for (int c = 0; c < 16; ++c) sc[kt][c] = left >= kt * 32 + 8 * (c >> 2) + (c & 3) ? sc[kt][c] : -INFINITY;
         }
-        if (upper) __syncthreads();                                         // (the same barrier: every wave passes one per tile)
-        __builtin_amdgcn_s_setprio(1);
-        if (more && (t + 1) * KT <= w_hi) scores(t + 1);
-        if (mine) {
-            const char* v_lds = lds + (2 + ((t - t_lo) & 1)) * TILE_BYTES;
-            if (b_lo - t * KT < KT - 1) {
-                const unsigned long long keys = flag[(t - t_lo) & 3];
-                if (keys) {
+        float mt = sc[0][0];
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) mt = fmaxf(mt, sc[kt][c]);
+        mt = max_of_halves(mt) * a.scale_log2e;
+        if (__any(mt > m + LAZY)) {
+            const float mn = fmaxf(m, mt), al = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int c = 0; c < 16; ++c) acc[i][c] *= al;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        if (!PLAIN) {
+            // values that are not finite, of a tile that not every row sees whole: whatever its weight, such a one decides the sum
+            const unsigned long long keys = flag[(t - t_lo) & 3];
+            if (keys) {
 #pragma nounroll
-                    for (int k = 0; k < KT; ++k) {                          // whatever its weight, what is not finite decides the sum
-                        if (!(keys >> k & 1) || pos - t * KT < k) continue;
-                        bool here;
-                        const int col = min((t * KT + k) >> p.page_shift, p.width - 1);
-                        const T* v = (const T*)((const char*)a.v_pages + place(t, table[col], k, here)) + 4 * hf;
-                        if (!here) continue;
+                for (int k = 0; k < KT; ++k) {
+                    if (!(keys >> k & 1) || pos - t * KT < k) continue;
+                    bool here;
+                    const unsigned key = (unsigned)t * KT + k;
+                    const T* v = (const T*)(v_pool + place(key, table[min(key >> p.page_shift, (unsigned)p.width - 1)], here)) + 4 * hf;
+                    if (!here) continue;
 #pragma unroll
-                        for (int i = 0; i < DT; ++i)
+                    for (int i = 0; i < DT; ++i)
 #pragma unroll
-                            for (int c = 0; c < 16; c += 4) {
-                                typedef typename Vec<T, 4>::type V4;
-                                const V4 x = i * 32 + 2 * c + 4 * hf < Dh ? *(const V4*)(v + i * 32 + 2 * c) : V4{};
+                        for (int c = 0; c < 16; c += 4) {
+                            typedef typename Vec<T, 4>::type V4;
+                            const V4 x = i * 32 + 2 * c + 4 * hf < Dh ? *(const V4*)(v + i * 32 + 2 * c) : V4{};
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[i][c + e] += __builtin_isfinite((float)x[e]) ? 0.f : (float)x[e];
-                            }
-                    }
+                            for (int e = 0; e < 4; ++e) acc[i][c + e] += __builtin_isfinite((float)x[e]) ? 0.f : (float)x[e];
+                        }
                 }
             }
+        }
+        // ---- weights of 16 keys, and their values
+#pragma unroll
+        for (int k16 = 0; k16 < KT / 16; ++k16) {
+            float w[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) w[c] = exp2_hw(fmaf(sc[k16 >> 1][(k16 & 1) * 8 + c], a.scale_log2e, -ms));
             if constexpr (sizeof(T) == 2) {
+                V8 pf;                                                      // rounded to the tensors' type for the matrix instruction
 #pragma unroll
-                for (int k16 = 0; k16 < KT / 16; ++k16)
+                for (int c = 0; c < 8; ++c) pf[c] = (T)w[c];
 #pragma unroll
-                    for (int i = 0; i < DT; ++i) {
-                        const int row = k16 * 16 + 4 * hf + ((lane & 15) >> 2), c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), o = (lane & 1) * 8;
-                        s16x4 v[2] = {read_tr(v_lds + TL::template voff<32>(row, c) + o), read_tr(v_lds + TL::template voff<32>(row + 8, c) + o)};
-                        acc[i] = mma32(__builtin_bit_cast(V8, v), pf[k16], acc[i]);
-                    }
-                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+                for (int c = 0; c < 8; c += 2) l = sum2(pf[c], pf[c + 1], w[c], w[c + 1], l);
 #pragma unroll
-                for (int i = 0; i < KT / 16 * DT - 4; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
-                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                for (int i = 0; i < DT; ++i) {
+                    const int rw = k16 * 16 + 4 * hf + ((lane & 15) >> 2), c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), o = (lane & 1) * 8;
+                    s16x4 v[2] = {read_tr(v_lds + TL::template voff<32>(rw, c) + o), read_tr(v_lds + TL::template voff<32>(rw + 8, c) + o)};
+                    acc[i] = mma32(__builtin_bit_cast(V8, v), pf, acc[i]);
+                }
             } else {
 #pragma unroll
-                for (int kt = 0; kt < NK; ++kt)
+                for (int c = 0; c < 8; ++c) l += w[c];
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const int row = kt * 32 + 8 * (c >> 2) + 4 * hf + (c & 3);
+                for (int c = 0; c < 8; ++c) {
+                    const int rw = k16 * 16 + 8 * (c >> 2) + 4 * hf + (c & 3);
 #pragma unroll
-                        for (int i = 0; i < DT; ++i)
-                            acc[i] = mma32(*(const float*)(v_lds + TL::template voff<32>(row, 8 * i + (l31 >> 2)) + (l31 & 3) * 4), pw[kt][c], acc[i]);
-                    }
+                    for (int i = 0; i < DT; ++i)
+                        acc[i] = mma32(*(const float*)(v_lds + TL::template voff<32>(rw, 8 * i + (l31 >> 2)) + (l31 & 3) * 4), w[c], acc[i]);
+                }
             }
         }
-        __builtin_amdgcn_s_setprio(0);
-        store_k(t + 2);
+        store_k(t + 1);
         store_v(t + 1);
+        __syncthreads();
+    };
+    if (tid < 4) { flag[tid] = 0; badf[tid] = 0; }
+    __syncthreads();
+    int t = t_lo;
+    if (t_lo < t_hi) {
+        look(t_lo);
+        load(t_lo);
+        store_k(t_lo);
+        store_v(t_lo);
     }
+    __syncthreads();
+    // first the tiles that every row of the block sees whole, then the rest (and what follows a missing page)
+    for (const int t_plain = min(t_hi, (b_lo + 1) / KT); t < t_plain; ++t) {
+        if (__builtin_amdgcn_readfirstlane(badf[(t - t_lo) & 3])) break;
+        tile(t, std::true_type{});
+    }
+    for (; t < t_hi; ++t) tile(t, std::false_type{});
     l += __shfl_xor(l, 32);
     if (r >= n_rows) return;
     const int64_t orow = (int64_t)(start + tok) * p.Hq + h;
@@ -691,16 +677,13 @@ __global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
 
 int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
-// Rows of a block: 32 per wave, as many as the streams have on average, fewer where the chip would not be filled
-int chunk_waves(const PagedArgs& p) {
-    const int64_t rows = (int64_t)p.M * (p.Hq / p.Hkv), per = rows / p.S;
-    const int64_t blocks8 = (rows / 256 + p.S) * p.Hkv;
-    return per > 128 && blocks8 >= 256 && padded_dim(p.Dh) <= 128 ? 8 : 4;
-}
-int64_t chunk_tiles(const PagedArgs& p, int nw) { return (int64_t)p.M * (p.Hq / p.Hkv) / (32 * nw) + p.S; }
-int chunk_splits(const PagedArgs& p, int elem, int nw) {
-    const int64_t blocks = chunk_tiles(p, nw) * p.Hkv, keys = (int64_t)p.width << p.page_shift;
-    int64_t s = blocks >= 512 ? 1 : 512 / blocks;
+int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
+// Parts of a row's keys: as many as fill the chip with blocks, of 256 keys at least (by the table's width: the lengths are on
+// the device).  A part costs a row (Dh + 2) floats written and read: little next to its fp32 products, so that there the blocks
+// may be cut finer for an even load; as much as 250 keys' 16-bit products, so that there no block is cut once every CU has two.
+int chunk_splits(const PagedArgs& p, int elem) {
+    const int64_t blocks = chunk_tiles(p) * p.Hkv, keys = (int64_t)p.width << p.page_shift, want = elem == ELEM_F32 ? 1280 : 512;
+    int64_t s = blocks >= want ? 1 : want / blocks;
     if (s > keys / 256) s = keys / 256;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
@@ -713,29 +696,25 @@ template <typename T, int DP> void run_one(AttendArgs a, hipStream_t s) {
     constexpr int keys = one_nw<DP>() * one_kt<T>();
     a.splits = !one_whole(p);
     attend_one<T, DP><<<a.splits ? ONE_GRID : (unsigned)segs, 64 * one_nw<DP>(), 0, s>>>(a);
-    if (a.splits) attend_join<T, DP><<<(unsigned)segs, DP, 0, s>>>(a, keys);
+    if (a.splits) attend_join<T, DP><<<dim3((unsigned)segs, (unsigned)(p.Hq / p.Hkv < ONE_ROWS ? p.Hq / p.Hkv : ONE_ROWS)), DP, 0, s>>>(a, keys);
 }
-template <typename T, int DP, int NW> void run_chunk_nw(AttendArgs a, hipStream_t s) {
+template <typename T, int DP> void run_chunk(AttendArgs a, hipStream_t s) {
     constexpr int bytes = 4 * chunk_kt<T>() * DP * (int)sizeof(T) + 48;
     static bool set[64];                                        // per device: more LDS than a kernel gets by default
     int dev = 0;
     (void)hipGetDevice(&dev);
     if (dev < 64 && !set[dev]) {
-        (void)hipFuncSetAttribute((const void*)attend_chunk<T, DP, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        (void)hipFuncSetAttribute((const void*)attend_chunk<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         set[dev] = true;
     }
-    const dim3 grid((unsigned)(chunk_tiles(a.p, NW) * a.p.Hkv), (unsigned)a.splits);
-    attend_chunk<T, DP, NW><<<grid, 64 * NW, bytes, s>>>(a);
+    const dim3 grid((unsigned)(chunk_tiles(a.p) * a.p.Hkv), (unsigned)a.splits);
+    attend_chunk<T, DP><<<grid, 64 * CHUNK_WAVES, bytes, s>>>(a);
     if (a.splits > 1) attend_chunk_join<T, DP><<<(unsigned)(((int64_t)a.p.M * a.p.Hq + 3) / 4), 256, 0, s>>>(a);
 }
 template <typename T, int DP> void run(AttendArgs a, int elem, hipStream_t s) {
     if (!a.p.offsets) { run_one<T, DP>(a, s); return; }
-    const int nw = chunk_waves(a.p);
-    a.splits = chunk_splits(a.p, elem, nw);
-    if constexpr (DP <= 128) {
-        if (nw == 8) { run_chunk_nw<T, DP, 8>(a, s); return; }
-    }
-    run_chunk_nw<T, DP, 4>(a, s);
+    a.splits = chunk_splits(a.p, elem);
+    run_chunk<T, DP>(a, s);
 }
 template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s) {
     switch (padded_dim(a.p.Dh)) {
@@ -750,7 +729,7 @@ template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s)
 int64_t attend_workspace(const AttendArgs& a, int elem) {
     const int DP = padded_dim(a.p.Dh);
     if (!a.p.offsets) return one_whole(a.p) ? 0 : (int64_t)ONE_GRID * 2 * piece_floats(DP) * (int64_t)sizeof(float);
-    const int n = chunk_splits(a.p, elem, chunk_waves(a.p));
+    const int n = chunk_splits(a.p, elem);
     return n > 1 ? (int64_t)n * a.p.M * a.p.Hq * (DP + 2) * (int64_t)sizeof(float) : 0;
 }
 void launch_attend(AttendArgs a, int elem, hipStream_t s) {
