@@ -22,8 +22,8 @@ from . import native
 _DTYPES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16IO}
 
 
-def _check(what, t, dtype, dev, shape):
-    """One tensor argument: type, device and shape (-1: any size)."""
+def _refuse(what, t, dtype, dev, shape):
+    """Says what is wrong with a tensor argument (-1 in shape: any size)."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError("%s must be a tensor" % what)
     if t.device != dev:
@@ -32,17 +32,27 @@ def _check(what, t, dtype, dev, shape):
         raise RuntimeError("%s must be %s, not %s" % (what, dtype, t.dtype))
     if len(t.shape) != len(shape) or any(b >= 0 and a != b for a, b in zip(t.shape, shape)):
         raise RuntimeError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple("any" if b < 0 else b for b in shape)))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s needs a gradient: the temporal operators are inference only" % what)
+    raise RuntimeError("%s needs a gradient: the temporal operators are inference only" % what)
 
 
-def _first(what, t):
+def _need(what, t, dtype, dev, shape):
+    """One tensor argument: type, device and shape, and no gradient.  (Single steps are bound by the host: this is their path.)"""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev.index) or \
+            (t.requires_grad and torch.is_grad_enabled()):
+        _refuse(what, t, dtype, dev, shape)
+
+
+def _lead(what, t, ndim):
+    """The tensor that the others are checked against: -> (dtype code, device, dtype, shape)."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise RuntimeError("%s must be a HIP device tensor (no CPU fallback)" % what)
-    code = _DTYPES.get(t.dtype)
+    dtype, dev, shape = t.dtype, t.device, t.shape
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise RuntimeError("%s: unsupported dtype %s (float32 / float16 / bfloat16)" % (what, t.dtype))
-    return code
+        raise RuntimeError("%s: unsupported dtype %s (float32 / float16 / bfloat16)" % (what, dtype))
+    if len(shape) != ndim or (t.requires_grad and torch.is_grad_enabled()):
+        _refuse(what, t, dtype, dev, (-1,) * ndim)
+    return code, dev, dtype, shape
 
 
 def _dense_last(t):
@@ -57,14 +67,17 @@ def _rows(t):
     return t if s2 == 1 and s0 % per == 0 and s1 % per == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _call(entry, code, block, dev):
     """One native call on the tensors' device and its current stream."""
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch._C._cuda_getDevice() == dev.index:
-        rc = entry(code, block, stream)
+    index = dev.index
+    if _current_device() == index:
+        rc = entry(code, block, _stream_of(index))
     else:
         with torch.cuda.device(dev):
-            rc = entry(code, block, stream)
+            rc = entry(code, block, _stream_of(index))
     if rc:
         native.check(rc, entry.__name__)
 
@@ -78,26 +91,22 @@ def causal_conv(x, weight, bias=None, state=None, silu=True):
 
     ``x`` [B,T,D] (any strides between rows, e.g. a slice of a projection), ``weight`` [W,D] with W = 2..4, ``bias`` [D],
     ``state`` [B,W-1,D], all of one dtype.  Returns ``(y, new state)``; the new state is the last W-1 rows of ``xx``."""
-    code = _first("x", x)
-    dev, dt = x.device, x.dtype
-    _check("x", x, dt, dev, (-1, -1, -1))
-    B, T, D = x.shape
-    _check("weight", weight, dt, dev, (-1, D))
-    W = weight.shape[0]
+    code, dev, dt, (B, T, D) = _lead("x", x, 3)
+    W = len(weight) if isinstance(weight, torch.Tensor) and weight.ndim else -1
+    _need("weight", weight, dt, dev, (W, D))
     if not 2 <= W <= 4:
         raise RuntimeError("weight: the filter has 2 to 4 taps, not %d" % W)
     x, weight = _dense_last(x), weight.contiguous()
     bp = sp = 0
     if bias is not None:
-        _check("bias", bias, dt, dev, (D,))
+        _need("bias", bias, dt, dev, (D,))
         bias = bias.contiguous()
         bp = bias.data_ptr()
     if state is not None:
-        _check("state", state, dt, dev, (B, W - 1, D))
+        _need("state", state, dt, dev, (B, W - 1, D))
         state = state.contiguous()
         sp = state.data_ptr()
-    y = torch.empty((B, T, D), dtype=dt, device=dev)
-    new = torch.empty((B, W - 1, D), dtype=dt, device=dev)
+    y, new = x.new_empty((B, T, D)), x.new_empty((B, W - 1, D))
     sb, st, _ = x.stride()
     _call(native.lib().rvm_causal_conv, code,
           _CONV.pack(x.data_ptr(), weight.data_ptr(), bp, sp, y.data_ptr(), new.data_ptr(), sb, st, B, T, D, W, bool(silu)), dev)
@@ -114,38 +123,35 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
     ``x``, ``dt``, ``z`` [b,T,d] and ``B``, ``C`` [b,T,N] of one dtype (any strides between rows), N = 1..64; ``A`` [N,d],
     ``D`` [d], ``dt_bias`` [d] and ``state`` [b,N,d] (None: zeros) in fp32.  Returns ``(y, new state)``.  Without ``softplus``
     the step size is ``dt + dt_bias`` itself."""
-    code = _first("x", x)
-    dev, ty, f32 = x.device, x.dtype, torch.float32
-    _check("x", x, ty, dev, (-1, -1, -1))
-    nb, T, nd = x.shape
-    _check("dt", dt, ty, dev, (nb, T, nd))
-    _check("A", A, f32, dev, (-1, nd))
-    N = A.shape[0]
+    code, dev, ty, (nb, T, nd) = _lead("x", x, 3)
+    f32 = torch.float32
+    _need("dt", dt, ty, dev, (nb, T, nd))
+    N = len(A) if isinstance(A, torch.Tensor) and A.ndim else -1
+    _need("A", A, f32, dev, (N, nd))
     if not 1 <= N <= 64:
         raise RuntimeError("A: 1 to 64 states per channel, not %d" % N)
-    _check("B", B, ty, dev, (nb, T, N))
-    _check("C", C, ty, dev, (nb, T, N))
+    _need("B", B, ty, dev, (nb, T, N))
+    _need("C", C, ty, dev, (nb, T, N))
     x, dt, B, C, A = _dense_last(x), _dense_last(dt), _dense_last(B), _dense_last(C), A.contiguous()
     zp = z_sb = z_st = 0
     if z is not None:
-        _check("z", z, ty, dev, (nb, T, nd))
+        _need("z", z, ty, dev, (nb, T, nd))
         z = _dense_last(z)
         zp, (z_sb, z_st, _) = z.data_ptr(), z.stride()
     Dp = bp = hp = 0
     if D is not None:
-        _check("D", D, f32, dev, (nd,))
+        _need("D", D, f32, dev, (nd,))
         D = D.contiguous()
         Dp = D.data_ptr()
     if dt_bias is not None:
-        _check("dt_bias", dt_bias, f32, dev, (nd,))
+        _need("dt_bias", dt_bias, f32, dev, (nd,))
         dt_bias = dt_bias.contiguous()
         bp = dt_bias.data_ptr()
     if state is not None:
-        _check("state", state, f32, dev, (nb, N, nd))
+        _need("state", state, f32, dev, (nb, N, nd))
         state = state.contiguous()
         hp = state.data_ptr()
-    y = torch.empty((nb, T, nd), dtype=ty, device=dev)
-    new = torch.empty((nb, N, nd), dtype=f32, device=dev)
+    y, new = x.new_empty((nb, T, nd)), A.new_empty((nb, N, nd))
     L = native.lib()
     need = L.rvm_selective_scan_workspace(nb, T, nd, N)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
@@ -157,32 +163,33 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
     return y, new
 
 
-def _paged(first, cache, table, lengths, offsets, code_of):
-    """Checks of what append_kv and attend share; ``first`` is the tensor of the new rows."""
-    code = _first(code_of, first)
-    dev, dt = first.device, first.dtype
+def _paged(what, rows, cache, table, lengths, offsets):
+    """Checks of what append_kv and attend share; ``rows`` is the tensor of the new rows."""
+    code, dev, dt, (M, H, Dh) = _lead(what, rows, 3)
     if not (isinstance(cache, (tuple, list)) and len(cache) == 2):
         raise RuntimeError("cache must be the pair (key pages, value pages)")
     kp, vp = cache
-    _check(code_of, first, dt, dev, (-1, -1, -1))
-    _check("key pages", kp, dt, dev, (-1, -1, -1, first.shape[2]))
-    _check("value pages", vp, dt, dev, kp.shape)
+    P, Hkv, page, _ = kp.shape if isinstance(kp, torch.Tensor) and kp.ndim == 4 else (-1, -1, -1, -1)
+    _need("key pages", kp, dt, dev, (P, Hkv, page, Dh))
+    _need("value pages", vp, dt, dev, (P, Hkv, page, Dh))
     if not (kp.is_contiguous() and vp.is_contiguous()):
         raise RuntimeError("the pages must be dense")
-    _check("table", table, torch.int32, dev, (-1, -1))
-    S = table.shape[0]
-    _check("lengths", lengths, torch.int32, dev, (S,))
+    S, width = table.shape if isinstance(table, torch.Tensor) and table.ndim == 2 else (-1, -1)
+    _need("table", table, torch.int32, dev, (S, width))
+    _need("lengths", lengths, torch.int32, dev, (S,))
     if not (table.is_contiguous() and lengths.is_contiguous()):
         raise RuntimeError("table and lengths must be dense")
     op = 0
     if offsets is not None:
-        _check("offsets", offsets, torch.int32, dev, (S + 1,))
+        _need("offsets", offsets, torch.int32, dev, (S + 1,))
         if not offsets.is_contiguous():
             raise RuntimeError("offsets must be dense")
         op = offsets.data_ptr()
-    elif first.shape[0] != S:
-        raise RuntimeError("without offsets every stream has one row: %d rows for %d streams" % (first.shape[0], S))
-    return code, dev, dt, kp, vp, S, op
+    elif M != S:
+        raise RuntimeError("without offsets every stream has one row: %d rows for %d streams" % (M, S))
+    if M and not S:
+        raise RuntimeError("%d rows for no stream" % M)
+    return code, dev, dt, kp, vp, (M, S, H, Hkv, Dh, P, page, width), (table.data_ptr(), lengths.data_ptr(), op)
 
 
 _APPEND = struct.Struct("10P16q")
@@ -201,31 +208,29 @@ def append_kv(k, v, cache, table, lengths, offsets=None, freqs=None, q=None, int
 
     ``freqs`` (fp32, radians per position; None: no rotation) turns the first ``2 * len(freqs)`` dims, a multiple of 16: the
     pairs (i, i + len(freqs)), or (2i, 2i+1) with ``interleaved``."""
-    code, dev, dt, kp, vp, S, op = _paged(k, cache, table, lengths, offsets, "k")
-    M, Hkv, Dh = k.shape
-    P, hk, page, _ = kp.shape
-    _check("v", v, dt, dev, (M, Hkv, Dh))
-    if hk != Hkv:
-        raise RuntimeError("k has %d heads, the pages have %d" % (Hkv, hk))
+    code, dev, dt, kp, vp, (M, S, H, Hkv, Dh, P, page, width), meta = _paged("k", k, cache, table, lengths, offsets)
+    _need("v", v, dt, dev, (M, H, Dh))
+    if H != Hkv:
+        raise RuntimeError("k has %d heads, the pages have %d" % (H, Hkv))
     k, v = _rows(k), _rows(v)
-    rot = fp = qp = op_q = q_sm = q_sh = 0
+    rot = fp = qp = out_p = q_sm = q_sh = 0
     Hq, out = Hkv, None
     if freqs is not None:
-        _check("freqs", freqs, torch.float32, dev, (-1,))
+        n = freqs.numel() if isinstance(freqs, torch.Tensor) else -1
+        _need("freqs", freqs, torch.float32, dev, (n,))
         freqs = freqs.contiguous()
-        rot, fp = 2 * freqs.numel(), freqs.data_ptr()
+        rot, fp = 2 * n, freqs.data_ptr()
     if q is not None:
-        _check("q", q, dt, dev, (M, -1, Dh))
-        Hq = q.shape[1]
+        Hq = q.shape[1] if isinstance(q, torch.Tensor) and q.ndim == 3 else -1
+        _need("q", q, dt, dev, (M, Hq, Dh))
         q = _rows(q)
-        out = torch.empty((M, Hq, Dh), dtype=dt, device=dev)
-        qp, op_q, (q_sm, q_sh, _) = q.data_ptr(), out.data_ptr(), q.stride()
-    if M and not S:
-        raise RuntimeError("%d rows for no stream" % M)
-    ks, vs = k.stride(), v.stride()
+        out = k.new_empty((M, Hq, Dh))
+        qp, out_p, (q_sm, q_sh, _) = q.data_ptr(), out.data_ptr(), q.stride()
+    k_sm, k_sh, _ = k.stride()
+    v_sm, v_sh, _ = v.stride()
     _call(native.lib().rvm_append_kv, code,
-          _APPEND.pack(qp, k.data_ptr(), v.data_ptr(), op_q, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), lengths.data_ptr(), op, fp,
-                       q_sm, q_sh, ks[0], ks[1], vs[0], vs[1], M, S, Hq, Hkv, Dh, P, page, table.shape[1], rot, bool(interleaved)), dev)
+          _APPEND.pack(qp, k.data_ptr(), v.data_ptr(), out_p, kp.data_ptr(), vp.data_ptr(), *meta, fp, q_sm, q_sh, k_sm, k_sh, v_sm, v_sh,
+                       M, S, Hq, Hkv, Dh, P, page, width, rot, bool(interleaved)), dev)
     return out
 
 
@@ -239,21 +244,17 @@ def attend(q, cache, table, lengths, offsets=None, scale=None):
 
     A row with a negative position, or behind the last stream's rows, gives 0.  Pages outside the pool are not followed:
     a row that would read one gives NaN."""
-    code, dev, dt, kp, vp, S, op = _paged(q, cache, table, lengths, offsets, "q")
-    M, Hq, Dh = q.shape
-    P, Hkv, page, _ = kp.shape
-    if M and not S:
-        raise RuntimeError("%d rows for no stream" % M)
+    code, dev, dt, kp, vp, sizes, meta = _paged("q", q, cache, table, lengths, offsets)
+    M, S, Hq, Hkv, Dh, P, page, width = sizes
     q = _rows(q)
-    out = torch.empty((M, Hq, Dh), dtype=dt, device=dev)
+    out = q.new_empty((M, Hq, Dh))
     L = native.lib()
     scale = Dh ** -0.5 if scale is None else float(scale)
     sm, sh, _ = q.stride()
     head = (q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr())
-    tail = (table.data_ptr(), lengths.data_ptr(), op, sm, sh, M, S, Hq, Hkv, Dh, P, page, table.shape[1])
-    need = L.rvm_attend_workspace(code, _ATTEND.pack(*head, 0, *tail, 0, scale))
+    need = L.rvm_attend_workspace(code, _ATTEND.pack(*head, 0, *meta, sm, sh, *sizes, 0, scale))
     if need < 0:
         native.check(1, "rvm_attend_workspace")
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call(L.rvm_attend, code, _ATTEND.pack(*head, ws.data_ptr() if ws is not None else 0, *tail, need, scale), dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(L.rvm_attend, code, _ATTEND.pack(*head, ws.data_ptr() if need else 0, *meta, sm, sh, *sizes, need, scale), dev)
     return out
