@@ -91,12 +91,13 @@ template <typename T, int VEC> void run_conv(const CausalConvArgs& a, hipStream_
 // composes them over the block (the decay over a chunk is exp(A sum delta)): every chunk's first state within its block, and
 // the block's last.  FROM composes the blocks in front of it, then runs its chunks from there.
 enum ScanMode { SCAN_WHOLE, SCAN_ENDS, SCAN_FROM };
-constexpr int SCAN_WAVES = 8, SCAN_BATCH = 4;           // waves of a block where the time axis is cut; steps requested ahead
+constexpr int SCAN_BATCH = 4;                           // steps requested ahead
+constexpr int SCAN_WAVES = 8;                           // waves of a block where the time axis is cut (16: two thirds slower at 1021 steps)
 template <int MODE> constexpr int scan_waves() { return MODE == SCAN_WHOLE ? 2 : SCAN_WAVES; }
 template <int NP> constexpr int scan_occupancy() { return NP <= 16 ? 4 : NP <= 32 ? 3 : 2; }      // waves of a SIMD
 
 template <typename T, int NP, int MODE>
-__global__ __launch_bounds__(64 * scan_waves<MODE>(), scan_occupancy<NP>()) void selective_scan(ScanArgs a) {
+__global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) void selective_scan(ScanArgs a) {
     constexpr int TB = SCAN_BATCH, NV = MODE == SCAN_ENDS ? NP : 2 * NP, LD = (TB * NV + 63) / 64, W = scan_waves<MODE>();
     constexpr int BC = LD * 64, TAB = NP * 64;
     constexpr int LDS = MODE == SCAN_ENDS ? (W * (TAB + 64) > W * 2 * BC ? W * (TAB + 64) : W * 2 * BC) : MODE == SCAN_FROM ? W * 2 * BC + TAB : W * 2 * BC;
@@ -145,28 +146,37 @@ __global__ __launch_bounds__(64 * scan_waves<MODE>(), scan_occupancy<NP>()) void
     const int64_t slot = (b * a.chunks + ch) * (int64_t)a.nD;           // of this chunk in carry and steps
     float steps = 0.f;
     if (MODE == SCAN_FROM) {
-        // the block's first state: a thread takes (n, channel) pairs and composes the blocks in front, eight requests at a time
+        // the block's first state: a thread takes (n, channel) pairs and composes the blocks in front, requested eight at a time
         float* H = lds + W * 2 * BC;
         const int64_t per = (int64_t)a.nD * (a.N + 1);
         const float* tot = a.totals + (b * gridDim.y) * per + d;        // per block: N rows of last states, a row of step sums
-        for (int n = wave; n < NP; n += W) {
-            const int nn = min(n, a.N - 1);
-            const float A2n = a.A[(int64_t)nn * a.nD + d] * LOG2E;
-            float hb = first ? first[(int64_t)nn * a.nD + d] : 0.f;
-            constexpr int U = 8;
-            for (int k0 = 0; k0 < (int)blockIdx.y; k0 += U) {
-                float e[U], st[U];
+        constexpr int NB = (NP + W - 1) / W, U = 8;
+        float hb[NB], A2n[NB];
+        int64_t row[NB];
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const float* at = tot + min(k0 + k, (int)blockIdx.y - 1) * per;
-                    e[k] = at[(int64_t)nn * a.nD]; st[k] = at[(int64_t)a.N * a.nD];
-                }
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (k0 + k < (int)blockIdx.y) hb = fmaf(exp2_hw(st[k] * A2n), hb, e[k]);
-            }
-            H[n * 64 + lane] = hb;
+        for (int k = 0; k < NB; ++k) {
+            row[k] = (int64_t)min(wave + k * W, a.N - 1) * a.nD;
+            A2n[k] = a.A[row[k] + d] * LOG2E;
+            hb[k] = first ? first[row[k] + d] : 0.f;
         }
+        for (int j0 = 0; j0 < (int)blockIdx.y; j0 += U) {
+            float e[U][NB], st[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float* at = tot + min(j0 + u, (int)blockIdx.y - 1) * per;
+                st[u] = at[(int64_t)a.N * a.nD];
+#pragma unroll
+                for (int k = 0; k < NB; ++k) e[u][k] = at[row[k]];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u < (int)blockIdx.y)
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) hb[k] = fmaf(exp2_hw(st[u] * A2n[k]), hb[k], e[u][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+            if (wave + k * W < NP) H[(wave + k * W) * 64 + lane] = hb[k];
         const float before = a.steps[slot + d];
 #pragma unroll
         for (int n = 0; n < NP; ++n) h[n] = a.carry[slot * a.N + (int64_t)min(n, a.N - 1) * a.nD + d];
@@ -296,13 +306,14 @@ void launch_causal_conv(const CausalConvArgs& a0, int elem, hipStream_t s) {
 }
 
 // Chunks of the time axis, a multiple of a block's waves: none where every SIMD has a wave without them, otherwise as many as
-// give it four waves (what the registers allow), of 16 steps at least
+// give it four waves (what the registers allow), of 8 steps at least
+constexpr int SCAN_MIN_STEPS = 8;
 int scan_chunks(int B, int T, int D) {
     const int64_t waves = (int64_t)B * ((D + 63) / 64), W = SCAN_WAVES;
     if (waves >= 1024 || T < 64) return 1;
     int64_t n = 4096 / waves / W * W;
-    if (n > T / 16 / W * W) n = T / 16 / W * W;
-    return n < W ? (T < 16 * W ? 1 : (int)W) : (int)n;
+    if (n > T / SCAN_MIN_STEPS / W * W) n = T / SCAN_MIN_STEPS / W * W;
+    return n < W ? (T < SCAN_MIN_STEPS * W ? 1 : (int)W) : (int)n;
 }
 int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N) {
     return B * (chunks + chunks / SCAN_WAVES) * (N + 1) * D;
@@ -310,7 +321,7 @@ int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N) {
 void launch_selective_scan(const ScanArgs& a0, int elem, hipStream_t s) {
     ScanArgs a = a0;
     a.dtiles = (a.nD + 63) / 64;
-    a.chunk_len = a.chunks > 1 ? ((a.T + a.chunks - 1) / a.chunks + 7) / 8 * 8 : a.T;
+    a.chunk_len = a.chunks > 1 ? ((a.T + a.chunks - 1) / a.chunks + SCAN_BATCH - 1) / SCAN_BATCH * SCAN_BATCH : a.T;
     a.steps = a.carry + (int64_t)a.B * a.chunks * a.N * a.nD;
     a.totals = a.steps + (int64_t)a.B * a.chunks * a.nD;
     if (elem == ELEM_F32) run_scan<float>(a, s);
