@@ -9,11 +9,11 @@ constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 // v * sigmoid(v); v_exp_f32 and v_rcp_f32 are good to one unit of the last place
 __device__ __forceinline__ float silu_f(float v) { return v * rcp_hw(1.f + exp2_hw(-LOG2E * v)); }
 // log(1 + e^v) = max(v, 0) + log1p(e^-|v|).  Step sizes are often 1e-3 and below, where log(1 + e) would keep three or four
-// digits of e: w = 1 + e is rounded, and log(w) e / (w - 1) puts back what the rounding took (the quotient varies slowly)
+// digits of e: w = 1 + e is rounded, and what the rounding took off e, at most half a unit of 1, is added back to log(w) (over w,
+// to be exact: 1 where e is small, and the term below a unit of the sum where it is not)
 __device__ __forceinline__ float softplus_f(float v) {
-    const float e = exp2_hw(-LOG2E * fabsf(v)), w = 1.f + e, d = w - 1.f;
-    const float lg = LN2 * __builtin_amdgcn_logf(w);
-    return fmaxf(v, 0.f) + (d == 0.f ? e : lg * e * rcp_hw(d));
+    const float e = exp2_hw(-LOG2E * fabsf(v)), w = 1.f + e;
+    return fmaxf(v, 0.f) + fmaf(LN2, __builtin_amdgcn_logf(w), e - (w - 1.f));
 }
 
 // ---- causal convolution: y[t] = act(bias + sum_w weight[w] xx[t + w]) with xx = the W-1 rows of the state, then x ----
@@ -111,31 +111,49 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
     const int d_own = dti * 64 + lane, d = min(d_own, a.nD - 1);
     const bool own = d_own < a.nD;
     const int t0 = MODE == SCAN_WHOLE ? 0 : min(a.T, ch * a.chunk_len), t1 = MODE == SCAN_WHOLE ? a.T : min(a.T, t0 + a.chunk_len);
-    const T* x = (const T*)a.x + b * a.x_sb + (int64_t)t0 * a.x_st + d;
-    const T* dt = (const T*)a.dt + b * a.dt_sb + (int64_t)t0 * a.dt_st + d;
-    const T* z = MODE != SCAN_ENDS && a.z ? (const T*)a.z + b * a.z_sb + (int64_t)t0 * a.z_st + d : nullptr;
+    // a wave's rows are at scalar addresses plus 4 bytes times the lane; B and C are dealt over the lanes, each with a pointer of its own
+    const char* x = (const char*)((const T*)a.x + b * a.x_sb + (int64_t)t0 * a.x_st);
+    const char* dt = (const char*)((const T*)a.dt + b * a.dt_sb + (int64_t)t0 * a.dt_st);
+    const char* z = MODE != SCAN_ENDS && a.z ? (const char*)((const T*)a.z + b * a.z_sb + (int64_t)t0 * a.z_st) : nullptr;
     const T* Bm = (const T*)a.Bm + b * a.B_sb + (int64_t)t0 * a.B_st;
     const T* Cm = (const T*)a.Cm + b * a.C_sb + (int64_t)t0 * a.C_st;
+    const unsigned off = d * (unsigned)sizeof(T);
+    const int64_t x_step = a.x_st * (int)sizeof(T), dt_step = a.dt_st * (int)sizeof(T), z_step = a.z_st * (int)sizeof(T);
     T xr[TB], dr[TB], zr[TB], br[LD];
+    const T* bp[LD];
+    int64_t b_inc[LD];
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+        const int e = j * 64 + lane, v = e % NV, n = min(v % NP, a.N - 1);
+        const int64_t st = v < NP ? a.B_st : a.C_st;
+        bp[j] = (v < NP ? Bm : Cm) + (e / NV) * st + n;
+        b_inc[j] = TB * st;
+    }
+    auto at = [&](const char* row) -> T { return *(const T*)(row + off); };
     auto load = [&](int left) {                         // the next `left` steps (TB or fewer: the last one again)
         if (left >= TB) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) { xr[i] = x[i * a.x_st]; dr[i] = dt[i * a.dt_st]; }
+            for (int i = 0; i < TB; ++i) { xr[i] = at(x + i * x_step); dr[i] = at(dt + i * dt_step); }
             if (z)
 #pragma unroll
-                for (int i = 0; i < TB; ++i) zr[i] = z[i * a.z_st];
+                for (int i = 0; i < TB; ++i) zr[i] = at(z + i * z_step);
+#pragma unroll
+            for (int j = 0; j < LD; ++j) { br[j] = *bp[j]; bp[j] += b_inc[j]; }
         } else {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) { const int64_t k = min(i, left - 1); xr[i] = x[k * a.x_st]; dr[i] = dt[k * a.dt_st]; if (z) zr[i] = z[k * a.z_st]; }
-        }
+            for (int i = 0; i < TB; ++i) {
+                const int64_t k = min(i, left - 1);
+                xr[i] = at(x + k * x_step); dr[i] = at(dt + k * dt_step);
+                if (z) zr[i] = at(z + k * z_step);
+            }
 #pragma unroll
-        for (int j = 0; j < LD; ++j) {
-            const int e = j * 64 + lane, v = e % NV, n = min(v % NP, a.N - 1);
-            const int64_t k = min(e / NV, left - 1);
-            br[j] = v < NP ? Bm[k * a.B_st + n] : Cm[k * a.C_st + n];
+            for (int j = 0; j < LD; ++j) {
+                const int k = (j * 64 + lane) / NV;
+                br[j] = k < left ? *bp[j] : (T)0.f;
+            }
         }
-        x += TB * a.x_st; dt += TB * a.dt_st; Bm += TB * a.B_st; Cm += TB * a.C_st;
-        if (z) z += TB * a.z_st;
+        x += TB * x_step; dt += TB * dt_step;
+        if (z) z += TB * z_step;
     };
     if (t0 < t1) load(t1 - t0);
     // ---- first states.  States past N: decay 1, input 0, start 0 - they stay 0
@@ -201,7 +219,8 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
         }
     }
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
-    T* y = (T*)a.y + (b * a.T + t0) * a.nD + d;
+    char* y = (char*)((T*)a.y + (b * a.T + t0) * a.nD);
+    const int64_t y_step = (int64_t)a.nD * (int)sizeof(T);
     int buf = 0;
     for (int t = t0; t < t1; t += TB, buf ^= 1) {
         float* bc = lds + (wave * 2 + buf) * BC;
@@ -231,7 +250,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
             }
             if (MODE != SCAN_ENDS) {
                 if (z) o *= silu_f(zv[i]);
-                if (own) y[(int64_t)(t - t0 + i) * a.nD] = (T)o;
+                if (own) *(T*)(y + i * y_step + off) = (T)o;
             }
         };
         if (t + TB <= t1) {
@@ -242,6 +261,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
             for (int i = 0; i < TB; ++i)
                 if (t + i < t1) step(i);
         }
+        y += TB * y_step;
     }
     if (MODE == SCAN_ENDS) {
         float* S = lds + W * TAB;                       // (the B values are done with)
