@@ -54,6 +54,10 @@ typedef const __attribute__((address_space(1))) u32x4* GlobalPiece;
 template <typename T> __device__ __forceinline__ u32x4 piece(const T* p, bool ok) {
     return *(ok ? (GlobalPiece)(uintptr_t)p : (GlobalPiece)(uintptr_t)&zero_piece);
 }
+// the same for what one block alone reads, once: not to be kept by the caches
+template <typename T> __device__ __forceinline__ u32x4 piece_once(const T* p, bool ok) {
+    return __builtin_nontemporal_load(ok ? (GlobalPiece)(uintptr_t)p : (GlobalPiece)(uintptr_t)&zero_piece);
+}
 
 // ---- one token per stream -------------------------------------------------------------------------------------------------
 // Work is cut by keys, not by streams: all streams' caches in units of NW tiles laid end to end, and block b of the grid
@@ -117,28 +121,25 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
     char* kt_lds = lds + wave * 2 * TILE_BYTES;
     char* vt_lds = kt_lds + TILE_BYTES;
 
+    // a stream without tokens has no unit: its row is 0
+    auto clear = [&](int s, int h0, int h1) {
+        for (int i = h0 * Dh + tid; i < h1 * Dh; i += 64 * NW) ((T*)a.out)[(int64_t)s * p.Hq * Dh + i] = (T)0.f;
+    };
     Units U;
-    U.sum(p, KEYS, segs);
     int64_t u0, u1;
-    if (a.splits) { u0 = blockIdx.x * U.per; u1 = min(U.total, u0 + U.per); }
-    else {                                                      // a block per segment, no pieces
-        const int s = blockIdx.x / segs;
-        int64_t before = 0;
-        for (int b = 0; b < s; b += 64) before += b + lane < s ? Units::of_stream(p, b + lane, KEYS) : 0;
-        for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
-        const int n = Units::of_stream(p, s, KEYS);
-        u0 = before * segs + (int64_t)(blockIdx.x % segs) * n; u1 = u0 + n;
-    }
-    // a stream without tokens (and its rows) has no unit: its rows are 0
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + tid; i < (int64_t)p.S * p.Hq; i += (int64_t)gridDim.x * blockDim.x) {
-        const int s = (int)(i / p.Hq);
-        if (p.lengths[s] < 0)
-            for (int d = 0; d < Dh; d += 8)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) ((T*)a.out)[i * Dh + d + k] = (T)0.f;
+    if (a.splits) {
+        U.sum(p, KEYS, segs);
+        u0 = blockIdx.x * U.per; u1 = min(U.total, u0 + U.per);
+        for (int s = blockIdx.x; s < p.S; s += gridDim.x)
+            if (p.lengths[s] < 0) clear(s, 0, p.Hq);
+    } else {                                                    // a block per segment, no pieces
+        U.stream = blockIdx.x / segs; U.first = 0; U.units = Units::of_stream(p, U.stream, KEYS);
+        const int seg = blockIdx.x - U.stream * segs;
+        u0 = (int64_t)seg * U.units; u1 = u0 + U.units;
+        if (!U.units && seg == 0) clear(U.stream, 0, p.Hq);
     }
     while (u0 < u1) {
-        U.find(p, KEYS, segs, u0);
+        if (a.splits) U.find(p, KEYS, segs, u0);
         const int s = __builtin_amdgcn_readfirstlane(U.stream), n_units = __builtin_amdgcn_readfirstlane(U.units);
         const int seg = (int)((u0 - U.first) / n_units);
         const int64_t seg0 = U.first + (int64_t)seg * n_units;
@@ -175,8 +176,8 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
                 lost |= !here && key <= (unsigned)pos;
                 const int64_t base = ((((int64_t)page * p.Hkv + kvh) << p.page_shift) + (key & page_mask)) * Dh;
                 const int kc = TL::kswz(row, pc) * TL::PER, vc = TL::template vswz<16>(row, pc) * TL::PER;
-                kr[j] = piece((const T*)a.k_pages + base + kc, ok && kc < Dh);
-                vr[j] = piece((const T*)a.v_pages + base + vc, ok && vc < Dh);
+                kr[j] = piece_once((const T*)a.k_pages + base + kc, ok && kc < Dh);
+                vr[j] = piece_once((const T*)a.v_pages + base + vc, ok && vc < Dh);
             }
         };
         int t = ua * NW + wave;

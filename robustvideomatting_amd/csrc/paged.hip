@@ -5,7 +5,8 @@ namespace {
 
 constexpr int APPEND_THREADS = 256, APPEND_MAX_ROT = 256;
 
-template <typename T, bool INTER>
+// ONCE: what is written does not fit the caches anyway and is written past them
+template <typename T, bool INTER, bool ONCE>
 __global__ __launch_bounds__(APPEND_THREADS) void append_kv(AppendArgs a) {
     typedef typename Vec<T, 8>::type V8;
     __shared__ float2 turn[APPEND_MAX_ROT / 2];
@@ -26,6 +27,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void append_kv(AppendArgs a) {
     const int nch = Dh >> 3, npair = a.rot >> 4;                // 16-byte pieces of a head; pairs of pieces that rotate together
     const int nq = a.q ? p.Hq : 0, items = INTER ? nch : nch - npair;
     const int64_t slot = pos & ((1 << p.page_shift) - 1);
+    auto put = [](T* to, V8 v) { if (ONCE) __builtin_nontemporal_store(v, (V8*)to); else *(V8*)to = v; };
     for (int i = tid; i < (nq + p.Hkv) * items; i += APPEND_THREADS) {
         const int h = i / items, c = i - h * items;
         const T* src; T* dst;
@@ -48,7 +50,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void append_kv(AppendArgs a) {
                 }
             }
             if (s >= p.S) v = V8{};                             // a row of no stream
-            *(V8*)(dst + c * 8) = v;
+            put(dst + c * 8, v);
         } else if (c < npair) {
             V8 u = *(const V8*)(src + c * 8), v = *(const V8*)(src + a.rot / 2 + c * 8);
 #pragma unroll
@@ -58,25 +60,31 @@ __global__ __launch_bounds__(APPEND_THREADS) void append_kv(AppendArgs a) {
                 u[j] = (T)(x * t.x - y * t.y); v[j] = (T)(x * t.y + y * t.x);
             }
             if (s >= p.S) u = v = V8{};
-            *(V8*)(dst + c * 8) = u;
-            *(V8*)(dst + a.rot / 2 + c * 8) = v;
+            put(dst + c * 8, u);
+            put(dst + a.rot / 2 + c * 8, v);
         } else {
             V8 v = *(const V8*)(src + (c + npair) * 8);
             if (s >= p.S) v = V8{};
-            *(V8*)(dst + (c + npair) * 8) = v;
+            put(dst + (c + npair) * 8, v);
         }
     }
     if (pg < 0) return;
     for (int i = tid; i < p.Hkv * nch; i += APPEND_THREADS) {
         const int h = i / nch, c = i - h * nch;
-        *(V8*)((T*)a.v_pages + ((((int64_t)pg * p.Hkv + h) << p.page_shift) + slot) * Dh + c * 8) =
-            *(const V8*)((const T*)a.v + m * a.v_sm + h * a.v_sh + c * 8);
+        put((T*)a.v_pages + ((((int64_t)pg * p.Hkv + h) << p.page_shift) + slot) * Dh + c * 8,
+            *(const V8*)((const T*)a.v + m * a.v_sm + h * a.v_sh + c * 8));
     }
 }
 
+template <typename T, bool ONCE> void run_append(const AppendArgs& a, hipStream_t s) {
+    if (a.interleaved) append_kv<T, true, ONCE><<<a.p.M, APPEND_THREADS, 0, s>>>(a);
+    else append_kv<T, false, ONCE><<<a.p.M, APPEND_THREADS, 0, s>>>(a);
+}
+// 21.6k tokens of 16 + 8 + 8 heads x 128 in bf16, 177 MB written: 64.5 us through the caches, 61.8 us past them.  Up to 32 MB
+// (the second-level caches together) what is appended may still be there when the attention reads it
 template <typename T> void run_append(const AppendArgs& a, hipStream_t s) {
-    if (a.interleaved) append_kv<T, true><<<a.p.M, APPEND_THREADS, 0, s>>>(a);
-    else append_kv<T, false><<<a.p.M, APPEND_THREADS, 0, s>>>(a);
+    const int64_t bytes = (int64_t)a.p.M * (2 * a.p.Hkv + (a.q ? a.p.Hq : 0)) * a.p.Dh * (int)sizeof(T);
+    if (bytes > (32 << 20)) run_append<T, true>(a, s); else run_append<T, false>(a, s);
 }
 
 }  // namespace

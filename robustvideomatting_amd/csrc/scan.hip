@@ -17,69 +17,76 @@ __device__ __forceinline__ float softplus_f(float v) {
 }
 
 // ---- causal convolution: y[t] = act(bias + sum_w weight[w] xx[t + w]) with xx = the W-1 rows of the state, then x ----
-constexpr int CONV_RUN = 16;                            // steps per thread: the W-1 rows before a run are read twice
-
-template <typename T, int VEC>
+// A thread has VEC channels (16 bytes) of RUN steps, taken four at a time with the next four requested ahead: the chip then
+// reads, computes and writes at the same time, where threads that request a whole run at once go through the three together.
+// The W-1 rows before a run are read again by the run before it (out of L2).
+template <typename T, int VEC, int RUN>
 __global__ __launch_bounds__(256) void causal_conv(CausalConvArgs a) {
     typedef typename Vec<T, VEC>::type V;
-    const int dv_n = a.D / VEC;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t bi = id / dv_n;
-    const int d = (int)(id - bi * dv_n) * VEC, run = (int)(bi % a.runs);
-    const int64_t b = bi / a.runs;
+    const unsigned dv_n = a.D / VEC, id = blockIdx.x * 256 + threadIdx.x, bi = id / dv_n;
+    const int d = (int)(id - bi * dv_n) * VEC;
+    const int64_t b = bi / (unsigned)a.runs;
+    const int run = (int)(bi - (unsigned)b * a.runs);
     if (b >= a.B) return;
-    const int W = a.W, t0 = run * CONV_RUN, t1 = min(a.T, t0 + CONV_RUN);
+    const int W = a.W, t0 = run * RUN;
     const T* x = (const T*)a.x + b * a.x_sb + d;
     const T* st = a.state_in ? (const T*)a.state_in + b * (W - 1) * a.D + d : nullptr;
-    auto row = [&](int i) -> V {                        // row i of xx
-        if (i >= W - 1) return *(const V*)(x + (int64_t)(i - (W - 1)) * a.x_st);
-        if (st) return *(const V*)(st + (int64_t)i * a.D);
+    auto row = [&](int t) -> V {                        // step t; the state's rows are steps -(W-1) .. -1
+        if (t >= 0) return *(const V*)(x + (int64_t)t * a.x_st);
+        if (st) return *(const V*)(st + (int64_t)(t + W - 1) * a.D);
         return V{};
     };
-    float w[4][VEC], win[4][VEC], bias[VEC];
+    constexpr int BT = RUN < 4 ? RUN : 4;
+    V in[BT + 3], next[BT], wt[4], bias = {};
+    auto rows = [&](V* to, int t) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < BT; ++k) to[k] = t + k < a.T ? row(t + k) : V{};
+    };
+    rows(next, t0);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) { w[k][j] = 0.f; win[k][j] = 0.f; }
-        if (k >= 4 - W) {                               // right-aligned: tap k of a shorter filter sits at k + 4 - W
-            const V v = *(const V*)((const T*)a.weight + (int64_t)(k - (4 - W)) * a.D + d);
+    for (int k = 0; k < 3; ++k) in[BT + k] = k >= 4 - W && t0 + k - 3 < a.T ? row(t0 + k - 3) : V{};
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[k][j] = (float)v[j];
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) bias[j] = a.bias ? (float)((const T*)a.bias)[d + j] : 0.f;
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-        if (k >= 4 - W) {
-            const V v = row(t0 + k - (4 - W));
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) win[k + 1][j] = (float)v[j];
-        }
+    for (int k = 0; k < 4; ++k)                         // right-aligned: tap k of a shorter filter sits at k + 4 - W
+        wt[k] = k >= 4 - W ? *(const V*)((const T*)a.weight + (int64_t)(k - (4 - W)) * a.D + d) : V{};
+    if (a.bias) bias = *(const V*)((const T*)a.bias + d);
     T* y = (T*)a.y + (b * a.T) * a.D + d;
-    for (int t = t0; t < t1; ++t) {
-        const V v = *(const V*)(x + (int64_t)t * a.x_st);
-        V o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            win[0][j] = win[1][j]; win[1][j] = win[2][j]; win[2][j] = win[3][j]; win[3][j] = (float)v[j];
-            float s = bias[j];
+    for (int c = 0; c < RUN; c += BT) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k >= 4 - W) s = fmaf(w[k][j], win[k][j], s);
-            o[j] = (T)(a.silu ? silu_f(s) : s);
-        }
-        *(V*)(y + (int64_t)t * a.D) = o;
+        for (int k = 0; k < 3; ++k) in[k] = in[BT + k];
+#pragma unroll
+        for (int k = 0; k < BT; ++k) in[k + 3] = next[k];
+        if (c + BT < RUN) rows(next, t0 + c + BT);
+#pragma unroll
+        for (int k = 0; k < BT; ++k)
+            if (t0 + c + k < a.T) {
+                V o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    float s = (float)bias[j];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        if (w >= 4 - W) s = fmaf((float)wt[w][j], (float)in[k + w][j], s);
+                    o[j] = (T)(a.silu ? silu_f(s) : s);
+                }
+                V* to = (V*)(y + (int64_t)(t0 + c + k) * a.D);
+                if (RUN > 1) __builtin_nontemporal_store(o, to); else *to = o;          // (past the caches: they are the rows' that are read twice)
+            }
     }
     if (run == a.runs - 1) {
         T* so = (T*)a.state_out + b * (W - 1) * a.D + d;
-        for (int k = 0; k < W - 1; ++k) *(V*)(so + (int64_t)k * a.D) = row(a.T + k);
+        for (int k = 0; k < W - 1; ++k) *(V*)(so + (int64_t)k * a.D) = row(a.T - (W - 1) + k);
     }
 }
 
-template <typename T, int VEC> void run_conv(const CausalConvArgs& a, hipStream_t s) {
+template <typename T, int VEC, int RUN> void run_conv_n(CausalConvArgs a, hipStream_t s) {
+    a.runs = a.T > RUN ? (a.T + RUN - 1) / RUN : 1;
     const int64_t n = (int64_t)a.B * a.runs * (a.D / VEC);
-    causal_conv<T, VEC><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    causal_conv<T, VEC, RUN><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+}
+// runs of 8 steps where there are as many, single steps otherwise
+template <typename T, int VEC> void run_conv(const CausalConvArgs& a, hipStream_t s) {
+    if (a.T < 8) run_conv_n<T, VEC, 1>(a, s); else run_conv_n<T, VEC, 8>(a, s);
 }
 
 // ---- selective scan: h_t = exp(delta_t A) h_(t-1) + delta_t x_t B_t,  y_t = C_t h_t + D x_t, times silu(z_t) ----
@@ -312,13 +319,11 @@ template <typename T> void run_scan(const ScanArgs& a, hipStream_t s) {
 
 }  // namespace
 
-void launch_causal_conv(const CausalConvArgs& a0, int elem, hipStream_t s) {
-    CausalConvArgs a = a0;
-    a.runs = a.T > 0 ? (a.T + CONV_RUN - 1) / CONV_RUN : 1;
+void launch_causal_conv(const CausalConvArgs& a, int elem, hipStream_t s) {
     const size_t es = elem == ELEM_F32 ? 4 : 2;
     const int vec = 16 / (int)es;
     auto ok = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-    const bool wide = a.D % vec == 0 && a.x_sb % vec == 0 && a.x_st % vec == 0 && ok(a.x) && ok(a.weight) && ok(a.state_in) &&
+    const bool wide = a.D % vec == 0 && a.x_sb % vec == 0 && a.x_st % vec == 0 && ok(a.x) && ok(a.weight) && ok(a.bias) && ok(a.state_in) &&
                       ok(a.y) && ok(a.state_out);
     if (elem == ELEM_F32) { if (wide) run_conv<float, 4>(a, s); else run_conv<float, 1>(a, s); }
     else if (elem == ELEM_F16) { if (wide) run_conv<f16, 8>(a, s); else run_conv<f16, 1>(a, s); }

@@ -57,7 +57,7 @@ int rvm_causal_conv(int dtype, const rvm_conv_args* c, void* hip_stream) {
     if (!c->B || !c->D) return 0;
     if (!c->weight || !c->state_out || (c->T && (!c->x || !c->y))) return fail(who, "null buffer");
     if (c->state_in == c->state_out) return fail(who, "state_out must not alias state_in");
-    if ((double)c->B * (c->T / 16 + 1) * c->D > 5e11) return fail(who, "too large for one launch");
+    if ((double)c->B * (c->T < 8 ? c->T + 1 : c->T / 8 + 1) * c->D > 4e9) return fail(who, "too large for one launch");
     CausalConvArgs a; memset(&a, 0, sizeof a);
     a.x = c->x; a.weight = c->weight; a.bias = c->bias; a.state_in = c->state_in; a.y = c->y; a.state_out = c->state_out;
     a.x_sb = c->x_sb; a.x_st = c->x_st; a.B = (int)c->B; a.T = (int)c->T; a.D = (int)c->D; a.W = (int)c->W; a.silu = c->silu != 0;
