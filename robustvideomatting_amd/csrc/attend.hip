@@ -679,13 +679,15 @@ __global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
 int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
 int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
-// Parts of a row's keys: as many as fill the chip with blocks, of 256 keys at least (by the table's width: the lengths are on
-// the device).  A part costs a row (Dh + 2) floats written and read: little next to its fp32 products, so that there the blocks
-// may be cut finer for an even load; as much as 250 keys' 16-bit products, so that there no block is cut once every CU has two.
+// Parts of a row's keys: as many as fill the chip with blocks, by the table's width (the lengths are on the device).  A part
+// costs a row (Dh + 2) floats written and read.  That is as much as 250 keys' 16-bit products: parts have 256 keys at least, and
+// no block is cut once every CU has two.  It is little next to fp32 products (a tile of 32 keys x 128 dims takes 4 us): 64 keys,
+// and the blocks may be cut finer for an even load.
 int chunk_splits(const PagedArgs& p, int elem) {
     const int64_t blocks = chunk_tiles(p) * p.Hkv, keys = (int64_t)p.width << p.page_shift, want = elem == ELEM_F32 ? 1280 : 512;
     int64_t s = blocks >= want ? 1 : want / blocks;
-    if (s > keys / 256) s = keys / 256;
+    const int64_t least = elem == ELEM_F32 ? 64 : 256;
+    if (s > keys / least) s = keys / least;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 // a cache that cannot hold more than this is not worth a second launch

@@ -13,6 +13,7 @@ Everything is channels-last.  Tensors are fp32, fp16 or bf16 on one HIP device; 
 fp32.  Work goes to the current stream of the tensors' device, nothing synchronises, every call can be captured into a HIP
 graph.  Inference only, like the network: tensors that need a gradient are refused.  No CPU fallback.
 """
+import functools
 import struct
 
 import torch
@@ -20,10 +21,15 @@ import torch
 from . import native
 
 _DTYPES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16IO}
+_F32, _I32 = torch.float32, torch.int32
+_grad = torch.is_grad_enabled
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _refuse(what, t, dtype, dev, shape):
-    """Says what is wrong with a tensor argument (-1 in shape: any size)."""
+# ---- arguments.  A call with a single step per stream is bound by the host, so each operator checks its arguments in one
+# expression; only a call that fails it comes here, to be told what is wrong
+def _tensor(what, t, dtype, dev, shape):
+    """One tensor argument: type, device and shape (-1: any size), and no gradient."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError("%s must be a tensor" % what)
     if t.device != dev:
@@ -32,27 +38,94 @@ def _refuse(what, t, dtype, dev, shape):
         raise RuntimeError("%s must be %s, not %s" % (what, dtype, t.dtype))
     if len(t.shape) != len(shape) or any(b >= 0 and a != b for a, b in zip(t.shape, shape)):
         raise RuntimeError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple("any" if b < 0 else b for b in shape)))
-    raise RuntimeError("%s needs a gradient: the temporal operators are inference only" % what)
+    if t.requires_grad and _grad():
+        raise RuntimeError("%s needs a gradient: the temporal operators are inference only" % what)
 
 
-def _need(what, t, dtype, dev, shape):
-    """One tensor argument: type, device and shape, and no gradient.  (Single steps are bound by the host: this is their path.)"""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev.index) or \
-            (t.requires_grad and torch.is_grad_enabled()):
-        _refuse(what, t, dtype, dev, shape)
-
-
-def _lead(what, t, ndim):
-    """The tensor that the others are checked against: -> (dtype code, device, dtype, shape)."""
+def _lead(what, t):
+    """The three-dimensional tensor that the others are checked against."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise RuntimeError("%s must be a HIP device tensor (no CPU fallback)" % what)
-    dtype, dev, shape = t.dtype, t.device, t.shape
-    code = _DTYPES.get(dtype)
-    if code is None:
-        raise RuntimeError("%s: unsupported dtype %s (float32 / float16 / bfloat16)" % (what, dtype))
-    if len(shape) != ndim or (t.requires_grad and torch.is_grad_enabled()):
-        _refuse(what, t, dtype, dev, (-1,) * ndim)
-    return code, dev, dtype, shape
+    if t.dtype not in _DTYPES:
+        raise RuntimeError("%s: unsupported dtype %s (float32 / float16 / bfloat16)" % (what, t.dtype))
+    _tensor(what, t, t.dtype, t.device, (-1, -1, -1))
+    return t.device, t.dtype, t.shape
+
+
+def _refuse_conv(x, weight, bias, state):
+    dev, dt, (B, T, D) = _lead("x", x)
+    _tensor("weight", weight, dt, dev, (-1, D))
+    W = weight.shape[0]
+    if not 2 <= W <= 4:
+        raise RuntimeError("weight: the filter has 2 to 4 taps, not %d" % W)
+    if bias is not None:
+        _tensor("bias", bias, dt, dev, (D,))
+    if state is not None:
+        _tensor("state", state, dt, dev, (B, W - 1, D))
+    raise RuntimeError("causal_conv: bad arguments")
+
+
+def _refuse_scan(x, dt, A, B, C, D, z, dt_bias, state):
+    dev, ty, (nb, T, nd) = _lead("x", x)
+    _tensor("dt", dt, ty, dev, (nb, T, nd))
+    _tensor("A", A, _F32, dev, (-1, nd))
+    N = A.shape[0]
+    if not 1 <= N <= 64:
+        raise RuntimeError("A: 1 to 64 states per channel, not %d" % N)
+    _tensor("B", B, ty, dev, (nb, T, N))
+    _tensor("C", C, ty, dev, (nb, T, N))
+    for what, t, kind, shape in (("z", z, ty, (nb, T, nd)), ("D", D, _F32, (nd,)), ("dt_bias", dt_bias, _F32, (nd,)), ("state", state, _F32, (nb, N, nd))):
+        if t is not None:
+            _tensor(what, t, kind, dev, shape)
+    raise RuntimeError("selective_scan: bad arguments")
+
+
+def _refuse_paged(what, rows, cache, table, lengths, offsets):
+    dev, dt, (M, H, Dh) = _lead(what, rows)
+    if not (isinstance(cache, (tuple, list)) and len(cache) == 2):
+        raise RuntimeError("cache must be the pair (key pages, value pages)")
+    kp, vp = cache
+    _tensor("key pages", kp, dt, dev, (-1, -1, -1, Dh))
+    _tensor("value pages", vp, dt, dev, kp.shape)
+    if not (kp.is_contiguous() and vp.is_contiguous()):
+        raise RuntimeError("the pages must be dense")
+    _tensor("table", table, _I32, dev, (-1, -1))
+    S = table.shape[0]
+    _tensor("lengths", lengths, _I32, dev, (S,))
+    if offsets is not None:
+        _tensor("offsets", offsets, _I32, dev, (S + 1,))
+    if not (table.is_contiguous() and lengths.is_contiguous() and (offsets is None or offsets.is_contiguous())):
+        raise RuntimeError("table, lengths and offsets must be dense")
+    if offsets is None and M != S:
+        raise RuntimeError("without offsets every stream has one row: %d rows for %d streams" % (M, S))
+    if M and not S:
+        raise RuntimeError("%d rows for no stream" % M)
+
+
+def _refuse_append(k, v, cache, table, lengths, offsets, freqs, q):
+    _refuse_paged("k", k, cache, table, lengths, offsets)
+    dev, dt, (M, H, Dh) = _lead("k", k)
+    _tensor("v", v, dt, dev, (M, H, Dh))
+    if H != cache[0].shape[1]:
+        raise RuntimeError("k has %d heads, the pages have %d" % (H, cache[0].shape[1]))
+    if freqs is not None:
+        _tensor("freqs", freqs, _F32, dev, (-1,))
+    if q is not None:
+        _tensor("q", q, dt, dev, (M, -1, Dh))
+    raise RuntimeError("append_kv: bad arguments")
+
+
+def _fits(rows, dt, di, kp, vp, table, lengths, offsets):
+    """Whether what append_kv and attend share is as it should be."""
+    M, _, Dh = rows.shape
+    S, _ = table.shape
+    P, Hkv, page, _ = shape = kp.shape
+    return (rows.is_cuda and shape == (P, Hkv, page, Dh) and vp.shape == shape and kp.dtype is dt and vp.dtype is dt and kp.get_device() == di and
+            vp.get_device() == di and kp.is_contiguous() and vp.is_contiguous() and table.dtype is _I32 and lengths.dtype is _I32 and
+            lengths.shape == (S,) and table.get_device() == di and lengths.get_device() == di and table.is_contiguous() and
+            lengths.is_contiguous() and (S or not M) and
+            (M == S if offsets is None else offsets.dtype is _I32 and offsets.shape == (S + 1,) and offsets.get_device() == di and offsets.is_contiguous()) and
+            not ((rows.requires_grad or kp.requires_grad or vp.requires_grad) and _grad()))
 
 
 def _dense_last(t):
@@ -67,16 +140,12 @@ def _rows(t):
     return t if s2 == 1 and s0 % per == 0 and s1 % per == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
-
-def _call(entry, code, block, dev):
+def _call(entry, code, block, index):
     """One native call on the tensors' device and its current stream."""
-    index = dev.index
     if _current_device() == index:
         rc = entry(code, block, _stream_of(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = entry(code, block, _stream_of(index))
     if rc:
         native.check(rc, entry.__name__)
@@ -91,29 +160,40 @@ def causal_conv(x, weight, bias=None, state=None, silu=True):
 
     ``x`` [B,T,D] (any strides between rows, e.g. a slice of a projection), ``weight`` [W,D] with W = 2..4, ``bias`` [D],
     ``state`` [B,W-1,D], all of one dtype.  Returns ``(y, new state)``; the new state is the last W-1 rows of ``xx``."""
-    code, dev, dt, (B, T, D) = _lead("x", x, 3)
-    W = len(weight) if isinstance(weight, torch.Tensor) and weight.ndim else -1
-    _need("weight", weight, dt, dev, (W, D))
-    if not 2 <= W <= 4:
-        raise RuntimeError("weight: the filter has 2 to 4 taps, not %d" % W)
+    try:
+        dt, di, (B, T, D), W = x.dtype, x.get_device(), x.shape, weight.shape[0]
+        ok = (x.is_cuda and dt in _DTYPES and weight.dtype is dt and weight.shape == (W, D) and weight.get_device() == di and 2 <= W <= 4 and
+              (bias is None or (bias.dtype is dt and bias.shape == (D,) and bias.get_device() == di)) and
+              (state is None or (state.dtype is dt and state.shape == (B, W - 1, D) and state.get_device() == di)) and
+              not (_grad() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                (state is not None and state.requires_grad))))
+    except (AttributeError, ValueError, IndexError):
+        ok = False
+    if not ok:
+        _refuse_conv(x, weight, bias, state)
     x, weight = _dense_last(x), weight.contiguous()
-    bp = sp = 0
     if bias is not None:
-        _need("bias", bias, dt, dev, (D,))
         bias = bias.contiguous()
-        bp = bias.data_ptr()
     if state is not None:
-        _need("state", state, dt, dev, (B, W - 1, D))
         state = state.contiguous()
-        sp = state.data_ptr()
     y, new = x.new_empty((B, T, D)), x.new_empty((B, W - 1, D))
     sb, st, _ = x.stride()
-    _call(native.lib().rvm_causal_conv, code,
-          _CONV.pack(x.data_ptr(), weight.data_ptr(), bp, sp, y.data_ptr(), new.data_ptr(), sb, st, B, T, D, W, bool(silu)), dev)
+    _call(native.lib().rvm_causal_conv, _DTYPES[dt],
+          _CONV.pack(x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if state is None else state.data_ptr(),
+                     y.data_ptr(), new.data_ptr(), sb, st, B, T, D, W, bool(silu)), di)
     return y, new
 
 
 _SCAN = struct.Struct("12P16q")
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_workspace(B, T, D, N):
+    """Bytes, by the sizes alone."""
+    need = native.lib().rvm_selective_scan_workspace(B, T, D, N)
+    if need < 0:
+        raise RuntimeError("selective_scan: bad shape")
+    return need
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, softplus=True):
@@ -123,73 +203,43 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
     ``x``, ``dt``, ``z`` [b,T,d] and ``B``, ``C`` [b,T,N] of one dtype (any strides between rows), N = 1..64; ``A`` [N,d],
     ``D`` [d], ``dt_bias`` [d] and ``state`` [b,N,d] (None: zeros) in fp32.  Returns ``(y, new state)``.  Without ``softplus``
     the step size is ``dt + dt_bias`` itself."""
-    code, dev, ty, (nb, T, nd) = _lead("x", x, 3)
-    f32 = torch.float32
-    _need("dt", dt, ty, dev, (nb, T, nd))
-    N = len(A) if isinstance(A, torch.Tensor) and A.ndim else -1
-    _need("A", A, f32, dev, (N, nd))
-    if not 1 <= N <= 64:
-        raise RuntimeError("A: 1 to 64 states per channel, not %d" % N)
-    _need("B", B, ty, dev, (nb, T, N))
-    _need("C", C, ty, dev, (nb, T, N))
+    try:
+        ty, di, xs, N = x.dtype, x.get_device(), x.shape, A.shape[0]
+        nb, T, nd = xs
+        bc = (nb, T, N)
+        ok = (x.is_cuda and ty in _DTYPES and dt.dtype is ty and dt.shape == xs and dt.get_device() == di and
+              A.dtype is _F32 and A.shape == (N, nd) and A.get_device() == di and 1 <= N <= 64 and
+              B.dtype is ty and B.shape == bc and B.get_device() == di and C.dtype is ty and C.shape == bc and C.get_device() == di and
+              (D is None or (D.dtype is _F32 and D.shape == (nd,) and D.get_device() == di)) and
+              (z is None or (z.dtype is ty and z.shape == xs and z.get_device() == di)) and
+              (dt_bias is None or (dt_bias.dtype is _F32 and dt_bias.shape == (nd,) and dt_bias.get_device() == di)) and
+              (state is None or (state.dtype is _F32 and state.shape == (nb, N, nd) and state.get_device() == di)) and
+              not (_grad() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, state))))
+    except (AttributeError, ValueError, IndexError):
+        ok = False
+    if not ok:
+        _refuse_scan(x, dt, A, B, C, D, z, dt_bias, state)
     x, dt, B, C, A = _dense_last(x), _dense_last(dt), _dense_last(B), _dense_last(C), A.contiguous()
     zp = z_sb = z_st = 0
     if z is not None:
-        _need("z", z, ty, dev, (nb, T, nd))
         z = _dense_last(z)
         zp, (z_sb, z_st, _) = z.data_ptr(), z.stride()
-    Dp = bp = hp = 0
     if D is not None:
-        _need("D", D, f32, dev, (nd,))
         D = D.contiguous()
-        Dp = D.data_ptr()
     if dt_bias is not None:
-        _need("dt_bias", dt_bias, f32, dev, (nd,))
         dt_bias = dt_bias.contiguous()
-        bp = dt_bias.data_ptr()
     if state is not None:
-        _need("state", state, f32, dev, (nb, N, nd))
         state = state.contiguous()
-        hp = state.data_ptr()
     y, new = x.new_empty((nb, T, nd)), A.new_empty((nb, N, nd))
-    L = native.lib()
-    need = L.rvm_selective_scan_workspace(nb, T, nd, N)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    need = _scan_workspace(nb, T, nd, N)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     xs, ds, Bs, Cs = x.stride(), dt.stride(), B.stride(), C.stride()
-    _call(L.rvm_selective_scan, code,
-          _SCAN.pack(x.data_ptr(), dt.data_ptr(), zp, B.data_ptr(), C.data_ptr(), A.data_ptr(), Dp, bp, hp, y.data_ptr(), new.data_ptr(),
-                     ws.data_ptr() if ws is not None else 0, xs[0], xs[1], ds[0], ds[1], z_sb, z_st, Bs[0], Bs[1], Cs[0], Cs[1],
-                     nb, T, nd, N, bool(softplus), need), dev)
+    _call(native.lib().rvm_selective_scan, _DTYPES[ty],
+          _SCAN.pack(x.data_ptr(), dt.data_ptr(), zp, B.data_ptr(), C.data_ptr(), A.data_ptr(), 0 if D is None else D.data_ptr(),
+                     0 if dt_bias is None else dt_bias.data_ptr(), 0 if state is None else state.data_ptr(), y.data_ptr(), new.data_ptr(),
+                     ws.data_ptr() if need else 0, xs[0], xs[1], ds[0], ds[1], z_sb, z_st, Bs[0], Bs[1], Cs[0], Cs[1],
+                     nb, T, nd, N, bool(softplus), need), di)
     return y, new
-
-
-def _paged(what, rows, cache, table, lengths, offsets):
-    """Checks of what append_kv and attend share; ``rows`` is the tensor of the new rows."""
-    code, dev, dt, (M, H, Dh) = _lead(what, rows, 3)
-    if not (isinstance(cache, (tuple, list)) and len(cache) == 2):
-        raise RuntimeError("cache must be the pair (key pages, value pages)")
-    kp, vp = cache
-    P, Hkv, page, _ = kp.shape if isinstance(kp, torch.Tensor) and kp.ndim == 4 else (-1, -1, -1, -1)
-    _need("key pages", kp, dt, dev, (P, Hkv, page, Dh))
-    _need("value pages", vp, dt, dev, (P, Hkv, page, Dh))
-    if not (kp.is_contiguous() and vp.is_contiguous()):
-        raise RuntimeError("the pages must be dense")
-    S, width = table.shape if isinstance(table, torch.Tensor) and table.ndim == 2 else (-1, -1)
-    _need("table", table, torch.int32, dev, (S, width))
-    _need("lengths", lengths, torch.int32, dev, (S,))
-    if not (table.is_contiguous() and lengths.is_contiguous()):
-        raise RuntimeError("table and lengths must be dense")
-    op = 0
-    if offsets is not None:
-        _need("offsets", offsets, torch.int32, dev, (S + 1,))
-        if not offsets.is_contiguous():
-            raise RuntimeError("offsets must be dense")
-        op = offsets.data_ptr()
-    elif M != S:
-        raise RuntimeError("without offsets every stream has one row: %d rows for %d streams" % (M, S))
-    if M and not S:
-        raise RuntimeError("%d rows for no stream" % M)
-    return code, dev, dt, kp, vp, (M, S, H, Hkv, Dh, P, page, width), (table.data_ptr(), lengths.data_ptr(), op)
 
 
 _APPEND = struct.Struct("10P16q")
@@ -208,33 +258,48 @@ def append_kv(k, v, cache, table, lengths, offsets=None, freqs=None, q=None, int
 
     ``freqs`` (fp32, radians per position; None: no rotation) turns the first ``2 * len(freqs)`` dims, a multiple of 16: the
     pairs (i, i + len(freqs)), or (2i, 2i+1) with ``interleaved``."""
-    code, dev, dt, kp, vp, (M, S, H, Hkv, Dh, P, page, width), meta = _paged("k", k, cache, table, lengths, offsets)
-    _need("v", v, dt, dev, (M, H, Dh))
-    if H != Hkv:
-        raise RuntimeError("k has %d heads, the pages have %d" % (H, Hkv))
+    try:
+        kp, vp = cache
+        dt, di, ks, qs = k.dtype, k.get_device(), k.shape, k.shape if q is None else q.shape
+        M, H, Dh = ks
+        ok = (dt in _DTYPES and _fits(k, dt, di, kp, vp, table, lengths, offsets) and kp.shape[1] == H and v.dtype is dt and v.shape == ks and
+              v.get_device() == di and (q is None or (q.dtype is dt and qs == (M, qs[1], Dh) and q.get_device() == di)) and
+              (freqs is None or (freqs.dtype is _F32 and freqs.dim() == 1 and freqs.get_device() == di)) and
+              not (_grad() and (v.requires_grad or (q is not None and q.requires_grad) or (freqs is not None and freqs.requires_grad))))
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    if not ok:
+        _refuse_append(k, v, cache, table, lengths, offsets, freqs, q)
     k, v = _rows(k), _rows(v)
     rot = fp = qp = out_p = q_sm = q_sh = 0
-    Hq, out = Hkv, None
+    out = None
     if freqs is not None:
-        n = freqs.numel() if isinstance(freqs, torch.Tensor) else -1
-        _need("freqs", freqs, torch.float32, dev, (n,))
         freqs = freqs.contiguous()
-        rot, fp = 2 * n, freqs.data_ptr()
+        rot, fp = 2 * freqs.shape[0], freqs.data_ptr()
     if q is not None:
-        Hq = q.shape[1] if isinstance(q, torch.Tensor) and q.ndim == 3 else -1
-        _need("q", q, dt, dev, (M, Hq, Dh))
         q = _rows(q)
-        out = k.new_empty((M, Hq, Dh))
+        out = k.new_empty(qs)
         qp, out_p, (q_sm, q_sh, _) = q.data_ptr(), out.data_ptr(), q.stride()
     k_sm, k_sh, _ = k.stride()
     v_sm, v_sh, _ = v.stride()
-    _call(native.lib().rvm_append_kv, code,
-          _APPEND.pack(qp, k.data_ptr(), v.data_ptr(), out_p, kp.data_ptr(), vp.data_ptr(), *meta, fp, q_sm, q_sh, k_sm, k_sh, v_sm, v_sh,
-                       M, S, Hq, Hkv, Dh, P, page, width, rot, bool(interleaved)), dev)
+    S, width = table.shape
+    _call(native.lib().rvm_append_kv, _DTYPES[dt],
+          _APPEND.pack(qp, k.data_ptr(), v.data_ptr(), out_p, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+                       0 if offsets is None else offsets.data_ptr(), fp, q_sm, q_sh, k_sm, k_sh, v_sm, v_sh,
+                       M, S, qs[1], H, Dh, kp.shape[0], kp.shape[2], width, rot, bool(interleaved)), di)
     return out
 
 
 _ATTEND = struct.Struct("8P11qd")
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(code, packed, *sizes):
+    """Bytes, by the sizes alone (``packed``: whether the rows come with offsets)."""
+    need = native.lib().rvm_attend_workspace(code, _ATTEND.pack(0, 0, 0, 0, 0, 16, 16, 16 * packed, 0, 0, *sizes, 0, 1.0))
+    if need < 0:
+        native.check(1, "rvm_attend_workspace")
+    return need
 
 
 def attend(q, cache, table, lengths, offsets=None, scale=None):
@@ -244,17 +309,26 @@ def attend(q, cache, table, lengths, offsets=None, scale=None):
 
     A row with a negative position, or behind the last stream's rows, gives 0.  Pages outside the pool are not followed:
     a row that would read one gives NaN."""
-    code, dev, dt, kp, vp, sizes, meta = _paged("q", q, cache, table, lengths, offsets)
-    M, S, Hq, Hkv, Dh, P, page, width = sizes
+    try:
+        kp, vp = cache
+        dt, di = q.dtype, q.get_device()
+        ok = dt in _DTYPES and _fits(q, dt, di, kp, vp, table, lengths, offsets)
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    if not ok:
+        _refuse_paged("q", q, cache, table, lengths, offsets)
+        raise RuntimeError("attend: bad arguments")
+    M, Hq, Dh = shape = q.shape
+    P, Hkv, page, _ = kp.shape
+    S, width = table.shape
+    code = _DTYPES[dt]
+    need = _attend_workspace(code, offsets is not None, M, S, Hq, Hkv, Dh, P, page, width)
     q = _rows(q)
-    out = q.new_empty((M, Hq, Dh))
-    L = native.lib()
-    scale = Dh ** -0.5 if scale is None else float(scale)
+    out = q.new_empty(shape)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     sm, sh, _ = q.stride()
-    head = (q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr())
-    need = L.rvm_attend_workspace(code, _ATTEND.pack(*head, 0, *meta, sm, sh, *sizes, 0, scale))
-    if need < 0:
-        native.check(1, "rvm_attend_workspace")
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(L.rvm_attend, code, _ATTEND.pack(*head, ws.data_ptr() if need else 0, *meta, sm, sh, *sizes, need, scale), dev)
+    _call(native.lib().rvm_attend, code,
+          _ATTEND.pack(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, table.data_ptr(),
+                       lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), sm, sh, M, S, Hq, Hkv, Dh, P, page, width, need,
+                       Dh ** -0.5 if scale is None else float(scale)), di)
     return out
