@@ -68,7 +68,7 @@ int rvm_causal_conv(int dtype, const rvm_conv_args* c, void* hip_stream) {
 int64_t rvm_selective_scan_workspace(int64_t B, int64_t T, int64_t D, int64_t N) {
     if (B < 0 || T < 0 || D < 0 || N < 1 || B > INT_LIMIT || T > INT_LIMIT || D > INT_LIMIT || N > 64) return -1;
     if (!B || !D) return 0;
-    const int64_t chunks = scan_chunks((int)B, (int)T, (int)D);
+    const int64_t chunks = scan_chunks((int)B, (int)T, (int)D, (int)N);
     return chunks > 1 ? scan_workspace_floats(B, chunks, D, N) * (int64_t)sizeof(float) : 0;
 }
 
@@ -91,7 +91,7 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
     a.x_sb = c->x_sb; a.x_st = c->x_st; a.dt_sb = c->dt_sb; a.dt_st = c->dt_st; a.z_sb = c->z_sb; a.z_st = c->z_st;
     a.B_sb = c->B_sb; a.B_st = c->B_st; a.C_sb = c->C_sb; a.C_st = c->C_st;
     a.B = (int)c->nB; a.T = (int)c->nT; a.nD = (int)c->nD; a.N = (int)c->nN; a.softplus = c->softplus != 0;
-    a.chunks = scan_chunks(a.B, a.T, a.nD);
+    a.chunks = scan_chunks(a.B, a.T, a.nD, a.N);
     a.carry = (float*)c->workspace;
     launch_selective_scan(a, elem, (hipStream_t)hip_stream);
     return launched(who);

@@ -27,7 +27,7 @@ struct ScanArgs {
     int B, T, nD, N, softplus, chunks, chunk_len, dtiles;
 };
 // how the time axis is split for this shape (1: not at all)
-int scan_chunks(int B, int T, int D);
+int scan_chunks(int B, int T, int D, int N);
 int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N);
 void launch_selective_scan(const ScanArgs& a, int elem, hipStream_t s);
 

@@ -157,6 +157,22 @@ def test_causal_conv(dtype, B, T, D, W, bias, state, silu, sliced):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D,front", [(20, 0), (20, 4), (26, 0), (26, 2), (40, 1), (40, 4), (64, 2)])
+def test_causal_conv_pieces(dtype, D, front):
+    """Channels and rows that begin on every kind of boundary: pieces of 16 bytes and fewer, single steps and runs."""
+    from robustvideomatting_amd import temporal as M
+    dt, g = DT[dtype], _gen(D + front)
+    for T in (1, 21):
+        x = _rn(g, 3, T, 2 * D, dtype=dt)[..., front:D + front]
+        w, b, s = _rn(g, 4, D, dtype=dt), _rn(g, D, dtype=dt), _rn(g, 3, 3, D, dtype=dt)
+        y, new = M.causal_conv(x, w, b, state=s)
+        (ry, rs), bound = O.causal_conv(x, w, b, s, True)
+        assert torch.equal(new.double(), rs)
+        _near(y, ry, O.rounded(ry, bound, dt), "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
 def test_a_chunk_equals_its_steps(dtype):
     """One call with T steps gives the bits of T calls with one step: convolution and scan."""
     from robustvideomatting_amd import temporal as M
@@ -208,6 +224,26 @@ def test_selective_scan(dtype, B, T, D, N, z, state, sliced):
     assert not state or torch.equal(h0, keep)
     again = M.selective_scan(x, step, A, Bm, Cm, Dv, zz, bias, h0)
     assert torch.equal(again[0], y) and torch.equal(again[1], h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("B,T,D,N,state,sliced", [
+    (4099, 1, 16, 16, True, False), (4098, 2, 20, 24, True, True), (1031, 40, 7, 8, True, True), (131, 300, 13, 16, True, True),
+    (67, 500, 31, 32, False, True), (133, 257, 32, 5, True, False), (1, 8160, 16, 16, True, False), (4097, 3, 1, 1, False, False),
+    (600, 64, 32, 64, True, False),
+])
+def test_selective_scan_of_many_narrow_sequences(dtype, B, T, D, N, state, sliced):
+    """Fewer channels than lanes and many sequences, whose number no group of them divides."""
+    from robustvideomatting_amd import temporal as M
+    dt, g = DT[dtype], _gen(B + T + D + N)
+    x, step, A, Bm, Cm, Dv, bias = _scan_inputs(g, B, T, D, N, dt, sliced)
+    zz = _rn(g, B, T, 2 * D, dtype=dt)[..., D:] if sliced else None
+    h0 = _rn(g, B, N, D) if state else None
+    y, h = M.selective_scan(x, step, A, Bm, Cm, Dv, zz, bias, h0)
+    (ry, rh), (by, bh) = O.selective_scan(x, step, A, Bm, Cm, Dv, zz, bias, h0)
+    _near(h, rh, bh + 1e-37, "state")
+    _near(y, ry, O.rounded(ry, by, dt), "y")
 
 
 @pytest.mark.gpu
