@@ -7,6 +7,7 @@
 //   attend_one    one new token per stream: the rows of a tile are the query heads that share a key head (16 x 16 tiles)
 //   attend_chunk  many rows per stream: (token, head of the group) pairs share every key they read (32 x 32 tiles)
 #include "temporal.hpp"
+#include <atomic>
 #include <type_traits>
 
 namespace {
@@ -76,7 +77,7 @@ struct Units {
     int64_t first;                      // first unit of that stream
     __device__ __forceinline__ static int of_stream(const PagedArgs& p, int s, int keys) {
         const int pos = s < p.S ? p.lengths[s] : -1;
-        return pos < 0 ? 0 : pos / keys + 1;
+        return pos < 0 ? 0 : (int)((paged_keys(p.width, p.page_shift, pos) - 1) / keys) + 1;
     }
     __device__ __forceinline__ void sum(const PagedArgs& p, int keys, int segs) {
         int64_t t = 0;
@@ -394,11 +395,11 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
     if (s < 0) return;
     row0 = __builtin_amdgcn_readfirstlane(row0); n_rows = __builtin_amdgcn_readfirstlane(n_rows); start = __builtin_amdgcn_readfirstlane(start);
     const int past = p.lengths[s];
-    auto at = [&](int token) { return (int)min((int64_t)INT32_MAX, max((int64_t)-1, (int64_t)past + token)); };
+    auto at = [&](int token) { return max(-1, paged_position(past, token)); };
     const int r = row0 + wave * 32 + l31, rr = min(r, n_rows - 1), tok = rr / group, h = kvh * group + rr - tok * group;
     const int pos = at(tok);                                                // this lane's row sees keys up to here
     const int b_lo = at(row0 / group), b_hi = at((min(row0 + R, n_rows) - 1) / group);
-    int t_lo = 0, t_hi = b_hi < 0 ? 0 : b_hi / KT + 1;
+    int t_lo = 0, t_hi = b_hi < 0 ? 0 : (int)((paged_keys(p.width, p.page_shift, b_hi) - 1) / KT) + 1;
     if (a.splits > 1) {
         const int per = (t_hi + a.splits - 1) / a.splits;
         t_lo = min(t_hi, (int)blockIdx.y * per); t_hi = min(t_hi, t_lo + per);
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
     }
     __syncthreads();
     // first the tiles that every row of the block sees whole, then the rest (and what follows a missing page)
-    for (const int t_plain = min(t_hi, (b_lo + 1) / KT); t < t_plain; ++t) {
+    for (const int t_plain = min(t_hi, (int)(((unsigned)b_lo + 1) / KT)); t < t_plain; ++t) {
         if (__builtin_amdgcn_readfirstlane(badf[(t - t_lo) & 3])) break;
         tile(t, std::true_type{});
     }
@@ -703,12 +704,12 @@ template <typename T, int DP> void run_one(AttendArgs a, hipStream_t s) {
 }
 template <typename T, int DP> void run_chunk(AttendArgs a, hipStream_t s) {
     constexpr int bytes = 4 * chunk_kt<T>() * DP * (int)sizeof(T) + 48;
-    static bool set[64];                                        // per device: more LDS than a kernel gets by default
+    static std::atomic<uint64_t> set;                           // devices (a bit each) that grant the kernel more LDS than the default
     int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (dev < 64 && !set[dev]) {
-        (void)hipFuncSetAttribute((const void*)attend_chunk<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        set[dev] = true;
+    if (hipGetDevice(&dev) != hipSuccess) return;               // (the error stays for the caller's check)
+    if (dev > 63 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (hipFuncSetAttribute((const void*)attend_chunk<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return;
+        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     const dim3 grid((unsigned)(chunk_tiles(a.p) * a.p.Hkv), (unsigned)a.splits);
     attend_chunk<T, DP><<<grid, 64 * CHUNK_WAVES, bytes, s>>>(a);

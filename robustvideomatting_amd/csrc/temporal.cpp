@@ -1,5 +1,5 @@
-// C entries of the temporal operators (include/rvm_mi355x.h): argument checks, then one launch each on the caller's stream
-// and the calling thread's current device.
+// C entries of the temporal operators (include/rvm_mi355x.h): argument checks, then one to three launches on the caller's
+// stream and the calling thread's current device.
 #include "temporal.hpp"
 #include "../../include/rvm_mi355x.h"
 
@@ -24,7 +24,7 @@ int elem_of(int dtype) {
         default: return -1;
     }
 }
-constexpr int64_t INT_LIMIT = 0x7fffffff;
+constexpr int64_t INT_LIMIT = 0x7fffffff, THREAD_LIMIT = 0xffffffff;     // of a launch, in one direction
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int paged_check(const char* who, PagedArgs& p, const int32_t* table, const int32_t* lengths, const int32_t* offsets, int64_t M, int64_t S,
@@ -35,6 +35,9 @@ int paged_check(const char* who, PagedArgs& p, const int32_t* table, const int32
     if (Dh < 8 || Dh > 256 || Dh % 8) return fail(who, "head size must be a multiple of 8, at most 256");
     if (page < 16 || page > 1024 || (page & (page - 1))) return fail(who, "page size must be a power of two from 16 to 1024");
     if (pages < 1 || pages > INT_LIMIT || width < 1 || width > INT_LIMIT || width * page > INT_LIMIT + 1) return fail(who, "bad page pool or table");
+    if (Hkv * page * Dh > INT_LIMIT / 4) return fail(who, "bad page pool or table: a page of all heads must stay below 2 GiB in fp32");
+    // what the kernels launch for M rows of S streams: at most 256 threads a row, a tile of 128 rows, or a (stream, key head, 16 heads)
+    if (M * 256 > THREAD_LIMIT || M * Hq > INT_LIMIT / 2 || S * Hkv * ((Hq / Hkv + 15) / 16) * 256 > THREAD_LIMIT / 2) return fail(who, "too large for one launch");
     if (M && S && (!table || !lengths)) return fail(who, "null table or lengths");
     memset(&p, 0, sizeof p);
     p.table = table; p.lengths = lengths; p.offsets = offsets;
@@ -81,7 +84,7 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
     if (c->nN < 1 || c->nN > 64) return fail(who, "1 to 64 states per channel");
     if (!c->nB || !c->nD) return 0;
     if (!c->A || !c->state_out || (c->nT && (!c->x || !c->dt || !c->B || !c->C || !c->y))) return fail(who, "null buffer");
-    if ((double)c->nB * ((c->nD + 63) / 64) > 1e9) return fail(who, "too large for one launch");
+    if (c->nB * ((c->nD + 63) / 64) > THREAD_LIMIT / 128) return fail(who, "too large for one launch");
     if (c->state_in == c->state_out) return fail(who, "state_out must not alias state_in");
     const int64_t need = rvm_selective_scan_workspace(c->nB, c->nT, c->nD, c->nN);
     if (need > 0 && (!c->workspace || c->workspace_bytes < need)) return fail(who, "workspace too small (rvm_selective_scan_workspace)");

@@ -69,7 +69,7 @@ __device__ __forceinline__ int paged_row(const PagedArgs& p, int m, int& pos) {
         if (s < p.S) i = m - p.offsets[s];
         if (i < 0) s = p.S;
     }
-    pos = s < p.S ? p.lengths[s] + i : -1;
+    pos = s < p.S ? paged_position(p.lengths[s], i) : -1;
     return s;
 }
 __device__ __forceinline__ int paged_page(const PagedArgs& p, int s, int pos) {

@@ -108,6 +108,42 @@ def test_c_entries_refuse_bad_arguments_before_any_launch(entry, base, change, t
     _refused(getattr(native.lib(), entry)(0, block, None), text)
 
 
+@pytest.mark.parametrize("entry,base,change,text", [
+    ("rvm_causal_conv", CONV_OK, dict(B=1 << 20, T=1 << 20), "too large"),
+    ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 26), "too large"),
+    ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 20, nD=1 << 20), "too large"),
+    ("rvm_append_kv", APPEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
+    ("rvm_append_kv", APPEND_OK, dict(Hkv=4096, Hq=4096, page=1024, Dh=256, pages=1), "below 2 GiB"),
+    ("rvm_attend", ATTEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
+    ("rvm_attend", ATTEND_OK, dict(M=1 << 20, S=8, offsets=4096, Hq=4096), "too large"),
+    ("rvm_attend", ATTEND_OK, dict(M=8, S=1 << 21, offsets=4096, Hq=8, Hkv=8), "too large"),
+    ("rvm_attend", ATTEND_OK, dict(M=1 << 20, S=1 << 20, Hq=1024), "too large"),
+    ("rvm_attend", ATTEND_OK, dict(Hkv=8192, Hq=8192, page=1024, Dh=128), "below 2 GiB"),
+])
+def test_c_entries_refuse_what_no_launch_holds(entry, base, change, text):
+    import struct
+    from robustvideomatting_amd import native
+    v = dict(base, **change)
+    assert set(v) == set(base)
+    block = struct.pack("%dqd" % (len(v) - 1) if "scale" in v else "%dq" % len(v), *v.values())
+    _refused(getattr(native.lib(), entry)(0, block, None), text)
+
+
+def test_positions_and_keys_stay_inside_an_int(tmp_path):
+    """A stream's positions saturate instead of wrapping round, and a pass over its keys ends one behind the table."""
+    src = tmp_path / "pos.cpp"
+    src.write_text('#include "%s/robustvideomatting_amd/csrc/paged_index.hpp"\nextern "C" int at(int l, int i) { return paged_position(l, i); }\n'
+                   'extern "C" unsigned keys(int w, int sh, int pos) { return paged_keys(w, sh, pos); }\n' % ROOT)
+    lib = tmp_path / "pos.so"
+    subprocess.check_call(["g++", "-O1", "-shared", "-fPIC", "-o", str(lib), str(src)])
+    f = ctypes.CDLL(str(lib))
+    f.keys.restype = ctypes.c_uint
+    top = 2 ** 31 - 1
+    assert [f.at(0, 0), f.at(7, 5), f.at(-3, 2), f.at(-3, 3), f.at(top, 0), f.at(top, 9), f.at(-top - 1, 0)] == [0, 12, -1, 0, top, top, -top - 1]
+    assert [f.keys(3, 4, p) for p in (0, 46, 47, 48, 100, top)] == [1, 47, 48, 49, 49, 49]
+    assert [f.keys(1 << 21, 10, p) for p in (0, top - 1, top)] == [1, top, top + 1]
+
+
 def test_c_entries_refuse_bad_types_and_null():
     from robustvideomatting_amd import native
     L = native.lib()
@@ -467,6 +503,67 @@ def test_attend_does_not_follow_bad_pages(new):
     got = M.attend(q, cache, table[:, :3].contiguous(), lens, None if one else torch.tensor(off, dtype=torch.int32).cuda())
     ref, bound = O.attend(q, *cache, [r[:3] for r in rows], lengths, None if one else off)
     _near(got, ref, O.rounded(ref, bound, torch.bfloat16), "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [2 ** 31 - 1, 5000])
+@pytest.mark.parametrize("width,per", [(8, 1), (60, 1), (8, 2), (60, 40)])
+def test_lengths_far_past_the_table(width, per, top):
+    """A length that no table holds costs no more than the table: its rows are NaN, the other streams' what they are."""
+    from robustvideomatting_amd import temporal as M
+    g, dt, lengths = _gen(6), torch.float16, [20, 30, 3]
+    cache, table, rows, lens = _attend_case(g, lengths, [per] * 3, 4, 2, 64, 16, dt, 0.0)
+    wide = torch.full((3, width), 0, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    off = None if per == 1 else torch.tensor(_offsets([per] * 3), dtype=torch.int32).cuda()
+    q, kv = _rn(g, 3 * per, 4, 64, dtype=dt), _rn(g, 3 * per, 2, 64, dtype=dt)
+    clean = M.attend(q, cache, wide, lens, off)
+    lens[1] = top
+    keep = [c.clone() for c in cache]
+    got = M.attend(q, cache, wide, lens, off)
+    mine = slice(per, 2 * per)
+    assert torch.isnan(got[mine]).all()
+    got[mine] = clean[mine]
+    assert torch.equal(got, clean)
+    lens[0] = lens[2] = -100
+    M.append_kv(kv, kv, cache, wide, lens, off)
+    assert torch.equal(cache[0], keep[0]) and torch.equal(cache[1], keep[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("longest", [60, 2500])
+def test_attend_many_streams_with_one_token(dtype, longest):
+    """More streams than a wave has lanes, some without a token, two tiles of query heads, in both forms."""
+    from robustvideomatting_amd import temporal as M
+    dt, g, S = DT[dtype], _gen(longest), 150
+    lengths = [(37 * i) % 61 - 8 for i in range(S)]
+    lengths[97] = longest
+    cache, table, rows, lens = _attend_case(g, lengths, [1] * S, 20, 1, 32, 16, dt, float("nan"))
+    q = _rn(g, S, 20, 32, dtype=dt)
+    got = M.attend(q, cache, table, lens)
+    ref, bound = O.attend(q, *cache, rows, lengths, None)
+    _near(got, ref, O.rounded(ref, bound, dt), "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_before_the_first_stream(dtype):
+    """Packed rows that begin and end with rows of no stream: they come out as 0 and store nothing."""
+    from robustvideomatting_amd import temporal as M
+    dt, g, lengths, off = DT[dtype], _gen(31), [5, 0, 100], [3, 10, 10, 45]
+    cache, table, rows, lens = _attend_case(g, lengths, [7, 0, 35], 4, 2, 64, 16, dt, 0.0)
+    offsets = torch.tensor(off, dtype=torch.int32).cuda()
+    q, k = _rn(g, 50, 4, 64, dtype=dt), _rn(g, 50, 2, 64, dtype=dt)
+    before = [c.clone() for c in cache]
+    qr = M.append_kv(k, k, cache, table, lens, offsets, q=q)
+    assert not qr[:3].any() and not qr[45:].any() and torch.equal(qr[3:45], q[3:45])
+    changed = [(c != b).any(-1).any(1).sum().item() for c, b in zip(cache, before)]
+    assert changed == [42, 42]
+    got = M.attend(qr, cache, table, lens, offsets)
+    ref, bound = O.attend(qr, *cache, rows, lengths, off)
+    assert not got[:3].any() and not got[45:].any()
+    _near(got, ref, O.rounded(ref, bound, dt), "out")
 
 
 @pytest.mark.gpu
