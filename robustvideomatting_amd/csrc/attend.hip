@@ -680,13 +680,14 @@ __global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
 int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
 int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
-// Parts of a row's keys: as many as fill the chip with blocks, by the table's width (the lengths are on the device).  A part
-// costs a row (Dh + 2) floats written and read.  That is as much as 250 keys' 16-bit products: parts have 256 keys at least, and
-// no block is cut once every CU has two.  It is little next to fp32 products (a tile of 32 keys x 128 dims takes 4 us): 64 keys,
-// and the blocks may be cut finer for an even load.
+// Parts of a row's keys, by the table's width (the lengths are on the device): none once every CU has its two blocks (16 streams
+// of 512 tokens, fp32: 79 us, 103 in two parts), otherwise as many as give that many blocks.  A part costs a row (Dh + 2) floats
+// written and read.  That is as much as 250 keys' 16-bit products: such parts have 256 keys at least.  It is little next to fp32
+// products (a tile of 32 keys x 128 dims takes 4 us): 64 keys, and 2.5 times the blocks, which evens out streams of different
+// lengths (510 tokens of 4 streams behind 1117 to 4080: 166 us, 229 with one round of blocks; behind 2000 each 119 and 102).
 int chunk_splits(const PagedArgs& p, int elem) {
-    const int64_t blocks = chunk_tiles(p) * p.Hkv, keys = (int64_t)p.width << p.page_shift, want = elem == ELEM_F32 ? 1280 : 512;
-    int64_t s = blocks >= want ? 1 : want / blocks;
+    const int64_t blocks = chunk_tiles(p) * p.Hkv, keys = (int64_t)p.width << p.page_shift;
+    int64_t s = blocks >= 512 ? 1 : (elem == ELEM_F32 ? 1280 : 512) / blocks;
     const int64_t least = elem == ELEM_F32 ? 64 : 256;
     if (s > keys / least) s = keys / least;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
