@@ -65,6 +65,8 @@ template <typename T> __device__ __forceinline__ u32x4 piece_once(const T* p, bo
 // takes the b-th equal share, whatever the streams' lengths - they are known on the device only.  A (stream, key head, 16 query
 // heads) segment that fits inside a share is finished there; the pieces of one that does not go to the workspace (a block
 // has at most two such pieces: its first and its last) and attend_join adds them up in order.
+// Bound by memory: 8 streams of 8 to 65 thousand tokens, 8 key heads x 128 in bf16, 1.08 GB, take 170 us and 7 of joining, 6.4 TB/s
+// (a large copy reads and writes 5.2).  Keys and values are read past the caches: 193 us through them.
 template <typename T> constexpr int one_kt() { return sizeof(T) == 2 ? 32 : 16; }         // keys per tile of a wave
 template <int DP> constexpr int one_nw() { return DP > 128 ? 2 : 4; }                      // waves of a block
 constexpr int ONE_ROWS = 16, ONE_GRID = 512;
@@ -329,7 +331,12 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // ---- many rows per stream -------------------------------------------------------------------------------------------------
 // A block's four waves have 32 rows each and share every tile of keys and values in LDS: two buffers, one barrier per tile, the
 // next tile requested at the start of a tile and stored at its end.  Inside a wave the exponentials of 16 keys run under the
-// matrix instructions of the 16 before them.
+// matrix instructions of the 16 before them.  The blocks of a stream walk the keys side by side, so that L2 serves 93 % of what
+// they read; equal shares of all the work, cut anywhere, would lose that (51 %) and 25 % of the speed.
+// Bound by instruction issue: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
+// with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
+// 409 us, 800 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 650 us,
+// 112 TF (154).  Two row sets per wave, or three waves per SIMD, spill; 32 keys per tile: 430 us.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
 
@@ -653,6 +660,11 @@ __global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
     const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (orow >= (int64_t)p.M * p.Hq) return;
     const int lane = threadIdx.x & 63;
+    // a lane's is one part (64 at most): their factors first, so that their rows are requested side by side
+    const float* first = a.part + orow * (DP + 2);
+    const int64_t step = (int64_t)p.M * p.Hq * (DP + 2);
+    const float* mine = first + min(lane, a.splits - 1) * step;
+    const float m = mine[DP], l = mine[DP + 1];                 // (rows of no stream: whatever is there, unused)
     int pos;
     const int s = paged_row(p, (int)(orow / p.Hq), pos);
     T* out = (T*)a.out + orow * p.Dh;
@@ -660,17 +672,27 @@ __global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
         for (int d = lane; d < p.Dh; d += 64) out[d] = (T)0.f;
         return;
     }
-    float M = -INFINITY, L = 0.f, acc[(DP + 63) / 64];
+    float M = m;
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float factor = lane < a.splits ? exp2_hw(m - (M == -INFINITY ? 0.f : M)) : 0.f;
+    float L = lane < a.splits ? l * factor : 0.f, acc[(DP + 63) / 64];
+    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
 #pragma unroll
     for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = 0.f;
-    for (int i = 0; i < a.splits; ++i) {
-        const float* o = a.part + ((int64_t)i * p.M * p.Hq + orow) * (DP + 2);
-        const float m = o[DP], l = o[DP + 1], mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
-        const float ea = exp2_hw(M - ms), eb = exp2_hw(m - ms);
+    constexpr int U = 4;
+    for (int i = 0; i < a.splits; i += U) {
+        float x[U][(DP + 63) / 64];
 #pragma unroll
-        for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = acc[k] * ea + o[min(lane + 64 * k, DP - 1)] * eb;
-        L = L * ea + l * eb;
-        M = mn;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < (DP + 63) / 64; ++k) x[u][k] = first[min(i + u, a.splits - 1) * step + lane + 64 * k];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float f = __shfl(factor, i + u);              // (i + u < 64 + U: past the last part it is not used)
+            if (i + u < a.splits)
+#pragma unroll
+                for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = fmaf(x[u][k], f, acc[k]);
+        }
     }
 #pragma unroll
     for (int k = 0; k < (DP + 63) / 64; ++k)
@@ -692,7 +714,8 @@ int chunk_splits(const PagedArgs& p, int elem) {
     if (s > keys / least) s = keys / least;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
-// a cache that cannot hold more than this is not worth a second launch
+// A cache that cannot hold more than this is not worth a second launch: 8 streams of 100 or 500 tokens, 8 heads on 2 x 64, take 8.9 us
+// with a block per segment and 13 in shares, of 1000 tokens 12 both ways, of 4000 35 and 13.
 bool one_whole(const PagedArgs& p) { return ((int64_t)p.width << p.page_shift) <= 512; }
 
 template <typename T, int DP> void run_one(AttendArgs a, hipStream_t s) {

@@ -5,6 +5,10 @@ namespace {
 
 constexpr int APPEND_THREADS = 256, APPEND_MAX_ROT = 256;
 
+// k' (a, b) = (a cos t - b sin t, a sin t + b cos t) with t = position x freqs[i], stored with v at the token's slot.  A block per
+// token, whose pieces are then all in flight at once and whose turns are computed once for all heads.  Bound by memory: 21.6k
+// tokens of 16 + 8 + 8 heads x 128 in bf16, 353 MB moved, take 60.7 us, 5.8 TB/s; 64 single tokens are a launch (3.4 us).
+// Sums of products in fp32, rounded once to the cache's type.
 // ONCE: what is written does not fit the caches anyway and is written past them
 template <typename T, bool INTER, bool ONCE>
 __global__ __launch_bounds__(APPEND_THREADS) void append_kv(AppendArgs a) {

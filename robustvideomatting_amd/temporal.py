@@ -1,7 +1,7 @@
 """Temporal operators on the GPU, beside the network's ConvGRU: the other two ways of carrying a stream's past.
 
-The reference's only memory of a stream is the ConvGRU state (/root/reference/model/decoder.py:152-190): these have no
-counterpart there.  They keep its contract (decoder.py:174-180): the caller owns the state, and one call with T steps gives
+The reference's only memory of a stream is the ConvGRU state (model/decoder.py:152-190): these have no
+counterpart there.  They keep its contract (model/decoder.py:174-180): the caller owns the state, and one call with T steps gives
 what T calls with one step give.
 
 * a state of fixed size: ``causal_conv`` (a short depthwise filter over time) and ``selective_scan`` (a state space scan with
