@@ -7,6 +7,7 @@
 //   attend_one    one new token per stream: the rows of a tile are the query heads that share a key head (16 x 16 tiles)
 //   attend_chunk  many rows per stream: (token, head of the group) pairs share every key they read (32 x 32 tiles)
 #include "temporal.hpp"
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -703,16 +704,17 @@ int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
 int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
 // Parts of a row's keys, by the table's width (the lengths are on the device): none once every CU has its two blocks (16 streams
-// of 512 tokens, fp32: 79 us, 103 in two parts), otherwise as many as give that many blocks.  A part costs a row (Dh + 2) floats
-// written and read.  That is as much as 250 keys' 16-bit products: such parts have 256 keys at least.  It is little next to fp32
-// products (a tile of 32 keys x 128 dims takes 4 us): 64 keys, and 2.5 times the blocks, which evens out streams of different
-// lengths (510 tokens of 4 streams behind 1117 to 4080: 166 us, 229 with one round of blocks; behind 2000 each 119 and 102).
+// of 512 tokens, fp32: 79 us, 103 in two parts), otherwise as many as come to that without beginning another round of blocks.  A
+// part costs a row (Dh + 2) floats written and read.  That is as much as 250 keys' 16-bit products: such parts have 256 keys at
+// least (64 tokens behind 2000, 8 heads on 2 x 128: 20 us, 25 with 512 keys), and a table of 1536 keys is not cut (2 streams of 512
+// tokens, 32 heads on 8 x 64: 16 us, 27 in two parts).  It is little next to fp32 products (a tile of 32 keys x 128 dims takes 4 us):
+// 64 keys, and two rounds of blocks, which even out streams of different lengths (510 tokens of 4 streams behind 1117 to 4080,
+// 8 heads on 2 x 64: 167 us, 183 with one round; behind 2000 each 109 and 102).
 int chunk_splits(const PagedArgs& p, int elem) {
-    const int64_t blocks = chunk_tiles(p) * p.Hkv, keys = (int64_t)p.width << p.page_shift;
-    int64_t s = blocks >= 512 ? 1 : (elem == ELEM_F32 ? 1280 : 512) / blocks;
-    const int64_t least = elem == ELEM_F32 ? 64 : 256;
-    if (s > keys / least) s = keys / least;
-    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+    const int64_t tiles = std::max<int64_t>(1, ((int64_t)p.M * (p.Hq / p.Hkv) + CHUNK_ROWS / 2) / CHUNK_ROWS), blocks = tiles * p.Hkv;
+    const int64_t keys = (int64_t)p.width << p.page_shift, least = elem == ELEM_F32 ? 64 : 256;
+    if (blocks >= 512 || (elem != ELEM_F32 && keys < 1536)) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(64, std::min(keys / least, (elem == ELEM_F32 ? 1024 : 512) / blocks)));
 }
 // A cache that cannot hold more than this is not worth a second launch: 8 streams of 100 or 500 tokens, 8 heads on 2 x 64, take 8.9 us
 // with a block per segment and 13 in shares, of 1000 tokens 12 both ways, of 4000 35 and 13.
