@@ -1,5 +1,6 @@
 // Causal convolution over time and selective state space scan, for chunks of steps and for single steps.
 #include "temporal.hpp"
+#include <algorithm>
 
 namespace {
 
@@ -366,7 +367,8 @@ void launch_causal_conv(const CausalConvArgs& a, int elem, hipStream_t s) {
 }
 
 // Chunks of the time axis, a multiple of a block's waves: none where every SIMD has a wave without them, otherwise as many as
-// give it four waves (what the registers allow), of 8 steps at least.  512 steps x 960 channels, bf16: 60 sequences 212 us in
+// give it four waves (what the registers allow), of 8 steps at least, or 12 where there are two waves per SIMD even so (3 x 1021
+// steps x 333, fp32: 29 us in 8, 25 in 12; 1 x 512 x 960, bf16: 18 and 21).  512 steps x 960 channels, bf16: 60 sequences 212 us in
 // chunks and 247 without, 70 sequences 247 and 249, 100 sequences 307 and 255.
 constexpr int SCAN_MIN_STEPS = 8;
 // Sequences of a wave: as many as its lanes hold (4 or 2: their B and C go through the same registers), where the chip has four
@@ -376,13 +378,15 @@ int scan_pack(int B, int T, int D, int N) {
     if (D > 32 || N > 32 || (T < 64 ? B : (int64_t)B * (T / SCAN_MIN_STEPS)) < 4096) return 1;
     return D <= 16 && N <= 16 ? 4 : 2;
 }
+// steps of a chunk: whole batches of loads
+int64_t scan_chunk_len(int64_t T, int64_t chunks) { return ((T + chunks - 1) / chunks + SCAN_BATCH - 1) / SCAN_BATCH * SCAN_BATCH; }
 int scan_chunks(int B, int T, int D, int N) {
     const int pack = scan_pack(B, T, D, N);
     const int64_t waves = ((int64_t)B + pack - 1) / pack * ((D + 63) / 64), W = SCAN_WAVES;
-    if (waves >= 1024 || T < 64) return 1;
-    int64_t n = 4096 / waves / W * W;
-    if (n > T / SCAN_MIN_STEPS / W * W) n = T / SCAN_MIN_STEPS / W * W;
-    return n < W ? (T < SCAN_MIN_STEPS * W ? 1 : (int)W) : (int)n;
+    if (waves >= 1024 || T < SCAN_MIN_STEPS * W) return 1;
+    const int64_t most = std::max(W, 4096 / waves / W * W), least = waves * (T / SCAN_MIN_STEPS) <= 2048 ? SCAN_MIN_STEPS : SCAN_MIN_STEPS + SCAN_BATCH;
+    const int64_t len = std::max(least, scan_chunk_len(T, most));
+    return (int)(((T + len - 1) / len + W - 1) / W * W);
 }
 int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N) {
     return B * (chunks + chunks / SCAN_WAVES) * (N + 1) * D;
@@ -390,7 +394,7 @@ int64_t scan_workspace_floats(int64_t B, int64_t chunks, int64_t D, int64_t N) {
 void launch_selective_scan(const ScanArgs& a0, int elem, hipStream_t s) {
     ScanArgs a = a0;
     a.dtiles = (a.nD + 63) / 64;
-    a.chunk_len = a.chunks > 1 ? ((a.T + a.chunks - 1) / a.chunks + SCAN_BATCH - 1) / SCAN_BATCH * SCAN_BATCH : a.T;
+    a.chunk_len = a.chunks > 1 ? (int)scan_chunk_len(a.T, a.chunks) : a.T;
     a.steps = a.carry + (int64_t)a.B * a.chunks * a.N * a.nD;
     a.totals = a.steps + (int64_t)a.B * a.chunks * a.nD;
     const int pack = scan_pack(a.B, a.T, a.nD, a.N);
