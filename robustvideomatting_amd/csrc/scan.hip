@@ -369,7 +369,8 @@ void launch_causal_conv(const CausalConvArgs& a, int elem, hipStream_t s) {
 // Chunks of the time axis, a multiple of a block's waves: none where every SIMD has a wave without them, otherwise as many as
 // give it four waves (what the registers allow), of 8 steps at least, or 12 where there are two waves per SIMD even so (3 x 1021
 // steps x 333, fp32: 29 us in 8, 25 in 12; 1 x 512 x 960, bf16: 18 and 21).  512 steps x 960 channels, bf16: 60 sequences 212 us in
-// chunks and 247 without, 70 sequences 247 and 249, 100 sequences 307 and 255.
+// chunks and 247 without, 70 sequences 247 and 249, 100 sequences 307 and 255.  16 sequences of 32 steps 17 in chunks and 16
+// without, of 48 steps 18 and 22; 40 of 63 steps 36 both ways.
 constexpr int SCAN_MIN_STEPS = 8;
 // Sequences of a wave: as many as its lanes hold (4 or 2: their B and C go through the same registers), where the chip has four
 // waves per SIMD even with a sequence each.  1000 x 200 steps x 16 channels, bf16, 16 states: 36 us against 95 with one each;
@@ -383,7 +384,7 @@ int64_t scan_chunk_len(int64_t T, int64_t chunks) { return ((T + chunks - 1) / c
 int scan_chunks(int B, int T, int D, int N) {
     const int pack = scan_pack(B, T, D, N);
     const int64_t waves = ((int64_t)B + pack - 1) / pack * ((D + 63) / 64), W = SCAN_WAVES;
-    if (waves >= 1024 || T < SCAN_MIN_STEPS * W) return 1;
+    if (waves >= 1024 || T < (waves > 512 ? 64 : 40)) return 1;
     const int64_t most = std::max(W, 4096 / waves / W * W), least = waves * (T / SCAN_MIN_STEPS) <= 2048 ? SCAN_MIN_STEPS : SCAN_MIN_STEPS + SCAN_BATCH;
     const int64_t len = std::max(least, scan_chunk_len(T, most));
     return (int)(((T + len - 1) / len + W - 1) / W * W);

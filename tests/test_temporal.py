@@ -283,6 +283,21 @@ def test_selective_scan_of_many_narrow_sequences(dtype, B, T, D, N, state, slice
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [39, 40, 41, 47, 63, 64, 65, 95, 96, 97])
+def test_selective_scan_around_the_first_chunks(T):
+    """Lengths at which the time axis begins to be cut, and chunks that are empty or shorter than the others."""
+    from robustvideomatting_amd import temporal as M
+    for B, D, N in ((2, 70, 16), (1, 33, 64), (550, 64, 8)):
+        g = _gen(T + B)
+        x, step, A, Bm, Cm, Dv, bias = _scan_inputs(g, B, T, D, N, torch.bfloat16, True)
+        h0 = _rn(g, B, N, D)
+        y, h = M.selective_scan(x, step, A, Bm, Cm, Dv, None, bias, h0)
+        (ry, rh), (by, bh) = O.selective_scan(x, step, A, Bm, Cm, Dv, None, bias, h0)
+        _near(h, rh, bh + 1e-37, "state")
+        _near(y, ry, O.rounded(ry, by, torch.bfloat16), "y")
+
+
+@pytest.mark.gpu
 def test_selective_scan_without_softplus_and_options():
     from robustvideomatting_amd import temporal as M
     g = _gen(3)
