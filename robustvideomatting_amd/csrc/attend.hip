@@ -336,8 +336,8 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // they read; equal shares of all the work, cut anywhere, would lose that (51 %) and 25 % of the speed.
 // Bound by instruction issue: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
 // with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
-// 409 us, 800 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 650 us,
-// 112 TF (154).  Two row sets per wave, or three waves per SIMD, spill; 32 keys per tile: 430 us.
+// 412 us, 790 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
+// 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.  Two row sets per wave, or three waves per SIMD, spill; 32 keys per tile: 430 us.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
 
