@@ -22,7 +22,7 @@ from . import native
 
 _DTYPES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16IO}
 _F32, _I32 = torch.float32, torch.int32
-_grad = torch.is_grad_enabled
+_grad, _empty_like = torch.is_grad_enabled, torch.empty_like
 _stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -140,6 +140,11 @@ def _rows(t):
     return t if s2 == 1 and s0 % per == 0 and s1 % per == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _dense_like(t):
+    """A new dense tensor of t's shape and type (``empty_like`` of a dense one: a quarter less of the host's time)."""
+    return _empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _call(entry, code, block, index):
     """One native call on the tensors' device and its current stream."""
     if _current_device() == index:
@@ -174,9 +179,12 @@ def causal_conv(x, weight, bias=None, state=None, silu=True):
     x, weight = _dense_last(x), weight.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    if state is not None:
+    if state is None:
+        new = x.new_empty((B, W - 1, D))
+    else:
         state = state.contiguous()
-    y, new = x.new_empty((B, T, D)), x.new_empty((B, W - 1, D))
+        new = _empty_like(state)
+    y = _dense_like(x)
     sb, st, _ = x.stride()
     _call(native.lib().rvm_causal_conv, _DTYPES[dt],
           _CONV.pack(x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if state is None else state.data_ptr(),
@@ -228,9 +236,12 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
         D = D.contiguous()
     if dt_bias is not None:
         dt_bias = dt_bias.contiguous()
-    if state is not None:
+    if state is None:
+        new = A.new_empty((nb, N, nd))
+    else:
         state = state.contiguous()
-    y, new = x.new_empty((nb, T, nd)), A.new_empty((nb, N, nd))
+        new = _empty_like(state)
+    y = _dense_like(x)
     need = _scan_workspace(nb, T, nd, N)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     xs, ds, Bs, Cs = x.stride(), dt.stride(), B.stride(), C.stride()
@@ -278,7 +289,7 @@ def append_kv(k, v, cache, table, lengths, offsets=None, freqs=None, q=None, int
         rot, fp = 2 * freqs.shape[0], freqs.data_ptr()
     if q is not None:
         q = _rows(q)
-        out = k.new_empty(qs)
+        out = _dense_like(q)
         qp, out_p, (q_sm, q_sh, _) = q.data_ptr(), out.data_ptr(), q.stride()
     k_sm, k_sh, _ = k.stride()
     v_sm, v_sh, _ = v.stride()
@@ -318,13 +329,13 @@ def attend(q, cache, table, lengths, offsets=None, scale=None):
     if not ok:
         _refuse_paged("q", q, cache, table, lengths, offsets)
         raise RuntimeError("attend: bad arguments")
-    M, Hq, Dh = shape = q.shape
+    M, Hq, Dh = q.shape
     P, Hkv, page, _ = kp.shape
     S, width = table.shape
     code = _DTYPES[dt]
     need = _attend_workspace(code, offsets is not None, M, S, Hq, Hkv, Dh, P, page, width)
     q = _rows(q)
-    out = q.new_empty(shape)
+    out = _dense_like(q)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     sm, sh, _ = q.stride()
     _call(native.lib().rvm_attend, code,
