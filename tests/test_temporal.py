@@ -119,6 +119,9 @@ def test_c_entries_refuse_bad_arguments_before_any_launch(entry, base, change, t
     ("rvm_attend", ATTEND_OK, dict(M=8, S=1 << 21, offsets=4096, Hq=8, Hkv=8), "too large"),
     ("rvm_attend", ATTEND_OK, dict(M=1 << 20, S=1 << 20, Hq=1024), "too large"),
     ("rvm_attend", ATTEND_OK, dict(Hkv=8192, Hq=8192, page=1024, Dh=128), "below 2 GiB"),
+    ("rvm_attend", ATTEND_OK, dict(width=64), "workspace"),
+    ("rvm_attend", ATTEND_OK, dict(width=64, offsets=4096), "workspace"),
+    ("rvm_attend", ATTEND_OK, dict(width=64, workspace=4104, workspace_bytes=1 << 40), "workspace"),
 ])
 def test_c_entries_refuse_what_no_launch_holds(entry, base, change, text):
     import struct
@@ -609,6 +612,95 @@ def test_frames_one_by_one_and_in_one_chunk():
         assert (part.double() - whole[:, sl].double()).abs().max() <= 4 * O.half_step(dt) * v.abs().max().item()
         lens2 += per
     assert torch.equal(cache[0], cache2[0]) and torch.equal(cache[1], cache2[1])
+
+
+@pytest.mark.gpu
+def test_pages_past_32_bits():
+    """A pool of more than 2^32 elements: its last pages hold what a small pool would."""
+    from robustvideomatting_amd import temporal as M
+    g, dt, Hkv, page, Dh = _gen(12), torch.float16, 2, 1024, 128
+    pages = (1 << 32) // (Hkv * page * Dh) + 40
+    lengths, new = [1500, 7, 3000], [1, 40, 300]
+    small, table, rows, lens = _attend_case(g, lengths, new, Hkv, Hkv, Dh, page, dt, 0.0)
+    n = small[0].shape[0]
+    big = tuple(torch.empty((pages, Hkv, page, Dh), dtype=dt, device="cuda") for _ in range(2))
+    for b, s in zip(big, small):
+        b[-n:] = s
+    far = torch.where(table < n, table + (pages - n), torch.full_like(table, -1))
+    assert big[0].numel() > 1 << 32
+    for per in (1, 2):                                      # packed rows, and a row per stream
+        off = torch.tensor(_offsets(new), dtype=torch.int32).cuda() if per == 1 else None
+        R = sum(new) if per == 1 else len(new)
+        q, k, v = (_rn(g, R, h, Dh, dtype=dt) for h in (4, Hkv, Hkv))
+        freqs = (10000.0 ** (-torch.arange(0, Dh, 2).float() / Dh)).cuda()
+        qs = M.append_kv(k, v, small, table, lens, off, freqs=freqs, q=q)
+        qb = M.append_kv(k, v, big, far, lens, off, freqs=freqs, q=q)
+        assert torch.equal(qs, qb) and torch.equal(big[0][-n:], small[0]) and torch.equal(big[1][-n:], small[1])
+        assert torch.equal(M.attend(qb, big, far, lens, off), M.attend(qs, small, table, lens, off))
+
+
+@pytest.mark.gpu
+def test_sequences_past_32_bits():
+    """Tensors of more than 2^31 elements: the last sequences are what they are alone."""
+    from robustvideomatting_amd import temporal as M
+    g, dt, B, T, D, N, last = _gen(13), torch.float16, 70000, 64, 512, 4, 1500
+    x, step, A, Bm, Cm, Dv, bias = _scan_inputs(g, last, T, D, N, dt)
+    w = _rn(g, 4, D, dtype=dt)
+    big = torch.zeros((B, T, D), dtype=dt, device="cuda")
+    assert big.numel() > 1 << 31
+    big[-last:] = x
+    y, state = M.causal_conv(big, w)
+    ys, ss = M.causal_conv(x, w)
+    assert torch.equal(y[-last:], ys) and torch.equal(state[-last:], ss)
+    b, c = (torch.zeros((B, T, N), dtype=dt, device="cuda") for _ in range(2))
+    b[-last:], c[-last:] = Bm, Cm
+    y, h = M.selective_scan(big, big, A, b, c, Dv, big, bias)
+    ys, hs = M.selective_scan(x, x, A, Bm, Cm, Dv, x, bias)
+    assert torch.equal(y[-last:], ys) and torch.equal(h[-last:], hs)
+    # one sequence: the tail continues from the state in front of it
+    flat = big.view(1, B * T, D)
+    y, _ = M.causal_conv(flat, w)
+    ys, _ = M.causal_conv(flat[:, -1000:], w, state=flat[:, -1003:-1000])
+    assert torch.equal(y[:, -1000:], ys)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_other_strides_and_orders(dtype):
+    """Time-major, broadcast, channel-strided and unaligned inputs give the bits of dense ones, and dense results."""
+    from robustvideomatting_amd import temporal as M
+    dt, g = DT[dtype], _gen(14)
+    B, T, D, N = 3, 70, 24, 16
+
+    def forms(t):
+        odd = torch.empty((*t.shape[:-1], 2 * t.shape[-1] + 1), dtype=t.dtype, device="cuda")
+        odd[..., 1::2] = t
+        return [t.transpose(0, 1).contiguous().transpose(0, 1), odd[..., 1::2], torch.cat([t[..., :1], t], -1)[..., 1:]]
+
+    x, step, A, Bm, Cm, Dv, bias = _scan_inputs(g, B, T, D, N, dt)
+    w, z = _rn(g, 4, D, dtype=dt), _rn(g, B, T, D, dtype=dt)
+    c0, s0 = M.causal_conv(x, w)
+    y0, h0 = M.selective_scan(x, step, A, Bm, Cm, Dv, z, bias)
+    for xx, ss, bb, cc, zz in zip(*(forms(t) for t in (x, step, Bm, Cm, z))):
+        c, s = M.causal_conv(xx, w.t().contiguous().t())
+        y, h = M.selective_scan(xx, ss, A.t().contiguous().t(), bb, cc, Dv, zz, bias)
+        assert torch.equal(c, c0) and torch.equal(s, s0) and torch.equal(y, y0) and torch.equal(h, h0)
+        assert all(t.is_contiguous() for t in (c, s, y, h))
+    one = [t[:1].expand(B, -1, -1) for t in (x, step, Bm, Cm, z)]       # the same sequence for all
+    y, h = M.selective_scan(*one[:2], A, *one[2:4], Dv, one[4], bias)
+    assert torch.equal(y, y0[:1].expand(B, -1, -1)) and torch.equal(h, h0[:1].expand(B, -1, -1))
+    cache, table, rows, lens = _attend_case(g, [20, 40, 0], [30, 1, 9], 2, 2, 32, 16, dt, 0.0)
+    off = torch.tensor([0, 30, 31, 40], dtype=torch.int32).cuda()
+    q, k = _rn(g, 40, 4, 32, dtype=dt), _rn(g, 40, 2, 32, dtype=dt)
+    freqs = (10000.0 ** (-torch.arange(0, 32, 2).float() / 32)).cuda()
+    r0 = M.append_kv(k, k, cache, table, lens, off, freqs=freqs, q=q)
+    o0, keep = M.attend(r0, cache, table, lens, off), [c.clone() for c in cache]
+    for qq, kk in zip(forms(q), forms(k)):
+        r = M.append_kv(kk, kk, cache, table, lens, off, freqs=torch.stack([freqs, freqs], 1)[:, 0], q=qq)
+        assert torch.equal(r, r0) and all(torch.equal(a, b) for a, b in zip(cache, keep))
+    for rr in forms(r0):
+        o = M.attend(rr, cache, table, lens, off)
+        assert torch.equal(o, o0) and o.is_contiguous()
 
 
 # ---- how they are called ----------------------------------------------------------------------------------------------
