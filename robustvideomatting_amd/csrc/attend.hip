@@ -354,6 +354,49 @@ __device__ __forceinline__ float sum2(bfl a, bfl b, float, float, float l) {
 
 constexpr int CHUNK_WAVES = 4, CHUNK_ROWS = 32 * CHUNK_WAVES;
 
+__device__ __forceinline__ int of_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+struct ChunkStream {
+    int start, rows, tiles, ahead;              // first packed row, rows, row tiles; keys before them, in those that a row tile adds
+    __device__ __forceinline__ ChunkStream(const PagedArgs& p, int s) : start(0), rows(0), tiles(0), ahead(0) {
+        if (s >= p.S) return;
+        const int lo = p.offsets[s], hi = p.offsets[s + 1], past = p.lengths[s], group = p.Hq / p.Hkv;
+        start = min(max(lo, 0), p.M);
+        rows = max(0, min(hi, p.M) - start);
+        tiles = (int)(((int64_t)rows * group + CHUNK_ROWS - 1) / CHUNK_ROWS);
+        ahead = (int)min((int64_t)1 << 29, min((int64_t)max(past, 0), (int64_t)p.width << p.page_shift) * group / CHUNK_ROWS);
+    }
+};
+// The row tiles of all streams by the keys they look at, the most first, so that what is left at the end are short ones: stream and
+// tile of the one in place `at` (-1: there are not so many).  A stream's tile t has ahead + t + 1 units of them.  Every lane counts
+// the tiles of at least so many units as its own threshold says, 64 thresholds at a time.  Run by a whole wave, a lane a stream.
+constexpr int LONGEST_FIRST = 16;               // streams, at most (each costs a few instructions per count)
+__device__ __forceinline__ int longest_first(const ChunkStream& c, int S, int at, int& tile) {
+    const int lane = threadIdx.x & 63;
+    auto count = [&](int units) {
+        int n = 0;
+        for (int s = 0; s < S; ++s) {
+            const int t = of_lane(c.tiles, s);
+            n += max(0, min(t, of_lane(c.ahead, s) + t + 1 - units));
+        }
+        return n;
+    };
+    int lo = 0, hi = 0;
+    for (int s = 0; s < S; ++s) hi = max(hi, of_lane(c.ahead, s) + of_lane(c.tiles, s));
+    if (__builtin_amdgcn_readfirstlane(count(0)) <= at) return -1;
+    while (lo < hi) {                           // more than `at` tiles have lo units, none has more than hi
+        const int step = (hi - lo) / 64 + 1, units = lo + lane * step;
+        const int b = 63 - __clzll(__ballot((count(units) > at) & (units <= hi)));
+        lo += b * step;
+        hi = min(hi, lo + step - 1);
+    }
+    int r = at - __builtin_amdgcn_readfirstlane(count(lo + 1));
+    unsigned long long of = __ballot(lane < S && c.ahead < lo && lo <= c.ahead + c.tiles);
+    while (r-- > 0) of &= of - 1;
+    const int s = __ffsll(of) - 1;
+    tile = lo - 1 - of_lane(c.ahead, s);
+    return s;
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2) void attend_chunk(AttendArgs a) {
     constexpr int KT = chunk_kt<T>(), NK = KT / 32, R = CHUNK_ROWS, NT = 64 * CHUNK_WAVES, DT = DP / 32;
@@ -375,27 +418,26 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
             for (int i = tid; i < p.Hq * Dh; i += NT) o[i] = (T)0.f;
         }
     }
-    // ---- stream and rows of this block: the streams' row tiles laid end to end, a stream's last (longest) tile first
+    // ---- stream and rows of this block
     int s = -1, row0 = 0, n_rows = 0, start = 0;
-    {
+    if (p.S <= LONGEST_FIRST) {
+        const ChunkStream c(p, lane);
+        int tile;
+        s = longest_first(c, p.S, tile_id, tile);
+        if (s >= 0) { start = of_lane(c.start, s); n_rows = of_lane(c.rows, s) * group; row0 = tile * R; }
+    } else {                                                                // the streams end to end, a stream's last (longest) tile first
         int64_t before = 0;
         for (int b = 0; b < p.S && s < 0; b += 64) {
-            int lo = 0, n = 0;
-            if (b + lane < p.S) {
-                lo = min(max(p.offsets[b + lane], 0), p.M);
-                n = max(0, min(p.offsets[b + lane + 1], p.M) - lo);
-            }
-            const int64_t mine = ((int64_t)n * group + R - 1) / R;
-            int64_t inc = mine;
+            const ChunkStream c(p, b + lane);
+            int64_t inc = c.tiles;
             for (int o = 1; o < 64; o <<= 1) { const int64_t v = __shfl_up(inc, o); if (lane >= o) inc += v; }
             const unsigned long long hit = __ballot(before + inc > tile_id);
             if (hit) {
                 const int l = __ffsll(hit) - 1;
-                const int64_t end = before + __shfl(inc, l);
                 s = b + l;
-                start = __shfl(lo, l);
-                n_rows = __shfl(n, l) * group;
-                row0 = (int)(end - 1 - tile_id) * R;
+                start = of_lane(c.start, l);
+                n_rows = of_lane(c.rows, l) * group;
+                row0 = (int)(before + __shfl(inc, l) - 1 - tile_id) * R;
             } else before += __shfl(inc, 63);
         }
     }
