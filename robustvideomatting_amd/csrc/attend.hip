@@ -352,7 +352,11 @@ __device__ __forceinline__ float sum2(bfl a, bfl b, float, float, float l) {
     return __builtin_amdgcn_fdot2_f32_bf16(B2{a, b}, B2{(bfl)1.f, (bfl)1.f}, l, false);   // two rounded weights in one instruction
 }
 
-constexpr int CHUNK_WAVES = 4, CHUNK_ROWS = 32 * CHUNK_WAVES;
+constexpr int CHUNK_WAVES = 4, CHUNK_ROWS = 32 * CHUNK_WAVES, CHUNK_EXTRA = 512;
+template <typename T> constexpr int chunk_start() { return sizeof(T) == 4 ? 256 : 384; }    // keys' worth of time that a block takes to start and end
+template <typename T> constexpr int chunk_least() { return sizeof(T) == 4 ? 64 : 256; }     // keys of a part, at least
+// floats of a piece: a row tile's sums as [DP / 4][rows][4], then its maxima and sums of weights
+constexpr int64_t chunk_piece(int DP) { return CHUNK_ROWS * (DP + 2); }
 
 __device__ __forceinline__ int of_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 struct ChunkStream {
@@ -366,36 +370,83 @@ struct ChunkStream {
         ahead = (int)min((int64_t)1 << 29, min((int64_t)max(past, 0), (int64_t)p.width << p.page_shift) * group / CHUNK_ROWS);
     }
 };
-// The row tiles of all streams by the keys they look at, the most first, so that what is left at the end are short ones: stream and
-// tile of the one in place `at` (-1: there are not so many).  A stream's tile t has ahead + t + 1 units of them.  Every lane counts
-// the tiles of at least so many units as its own threshold says, 64 thresholds at a time.  Run by a whole wave, a lane a stream.
-constexpr int LONGEST_FIRST = 16;               // streams, at most (each costs a few instructions per count)
-__device__ __forceinline__ int longest_first(const ChunkStream& c, int S, int at, int& tile) {
-    const int lane = threadIdx.x & 63;
-    auto count = [&](int units) {
+// The work of up to 64 streams: their row tiles by the keys they look at, the most first, and the long ones in parts.  A stream's
+// tile t has ahead + t + 1 units of keys; one of more than `part` units is cut, into level 0 .. of it.  Run by a whole wave, a lane a
+// stream; uniform results, which depend on the lengths alone.
+constexpr int CHUNK_STREAMS = 64, CHUNK_LEVELS = 64, CHUNK_SLOTS = 512;
+struct ChunkPlan {
+    const ChunkStream& c;
+    int S, part;
+    int level, upto;                            // lane j: tiles that have a part j; parts 1 to j of all tiles
+    // tiles of more than so many units (a lane's own number)
+    __device__ __forceinline__ int above(int units) const {
         int n = 0;
         for (int s = 0; s < S; ++s) {
             const int t = of_lane(c.tiles, s);
-            n += max(0, min(t, of_lane(c.ahead, s) + t + 1 - units));
+            n += max(0, min(t, of_lane(c.ahead, s) + t - units));
         }
         return n;
-    };
-    int lo = 0, hi = 0;
-    for (int s = 0; s < S; ++s) hi = max(hi, of_lane(c.ahead, s) + of_lane(c.tiles, s));
-    if (__builtin_amdgcn_readfirstlane(count(0)) <= at) return -1;
-    while (lo < hi) {                           // more than `at` tiles have lo units, none has more than hi
-        const int step = (hi - lo) / 64 + 1, units = lo + lane * step;
-        const int b = 63 - __clzll(__ballot((count(units) > at) & (units <= hi)));
-        lo += b * step;
-        hi = min(hi, lo + step - 1);
     }
-    int r = at - __builtin_amdgcn_readfirstlane(count(lo + 1));
-    unsigned long long of = __ballot(lane < S && c.ahead < lo && lo <= c.ahead + c.tiles);
-    while (r-- > 0) of &= of - 1;
-    const int s = __ffsll(of) - 1;
-    tile = lo - 1 - of_lane(c.ahead, s);
-    return s;
-}
+    // The length of a part, `least` at least: of 63 of them, a lane's each, from a slot's fair share to five, and no cut at all, the one
+    // that ends first - by the longest part where every part finds a slot at once, by the work of a slot and half a part where not -
+    // with `start` units for the beginning of each.  Shares this long give fewer than `extra` parts beyond the tiles' first ones.
+    __device__ __forceinline__ ChunkPlan(const ChunkStream& c, int S, int Hkv, int extra, int least, int start) : c(c), S(S), part(1 << 30) {
+        const int lane = threadIdx.x & 63;
+        if (extra) {
+            double all = 0, parts = 0;
+            int most = 1;
+            for (int s = 0; s < S; ++s) {
+                const int t = of_lane(c.tiles, s), a = of_lane(c.ahead, s);
+                all += (double)t * (a + 0.5 * (t + 1));
+                if (t) most = max(most, a + t);
+            }
+            all *= Hkv;
+            const double share = all / extra * (lane + 16) / 16;
+            const int floor = max(least, (most + CHUNK_LEVELS - 1) / CHUNK_LEVELS);
+            const unsigned mine = lane == 63 || share > most ? most : max(floor, (int)share + 1);
+            for (int s = 0; s < S; ++s) {       // of a stream, about: the shortest tile's and the longest's
+                const int t = of_lane(c.tiles, s), a = of_lane(c.ahead, s);
+                parts += 0.5 * t * ((a + t + mine - 1) / mine + (a + mine) / mine);
+            }
+            parts *= Hkv;
+            const double cost = parts <= CHUNK_SLOTS ? (double)mine + start : (all + parts * start) / CHUNK_SLOTS + 0.5 * mine;
+            double best = cost;
+            for (int o = 32; o; o >>= 1) best = fmin(best, __shfl_xor(best, o));
+            part = of_lane((int)mine, 63 - __clzll(__ballot(cost == best)));
+        }
+        level = above((int)min((int64_t)lane * part, (int64_t)1 << 30));
+        upto = lane ? level : 0;
+        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(upto, o); if (lane >= o) upto += v; }
+    }
+    __device__ __forceinline__ int tiles() const { return of_lane(level, 0); }
+    __device__ __forceinline__ int cut() const { return of_lane(level, 1); }          // tiles in parts: the first so many
+    __device__ __forceinline__ int beyond() const { return of_lane(upto, 63); }       // parts beyond the tiles' first ones
+    // part number and place of the tile of the b-th of them
+    __device__ __forceinline__ int part_of(int b, int& at) const {
+        const int j = __ffsll(__ballot(upto > b)) - 1;
+        at = b - of_lane(upto - level, j);
+        return j;
+    }
+    // the tile in place `at` < tiles(): its stream and number.  64 thresholds at a time
+    __device__ __forceinline__ int find(int at, int& tile) const {
+        const int lane = threadIdx.x & 63;
+        int lo = 0, hi = 0;                     // more than `at` tiles have over lo units, none has over hi
+        for (int s = 0; s < S; ++s) hi = max(hi, of_lane(c.ahead, s) + of_lane(c.tiles, s));
+        while (lo + 1 < hi) {
+            const int step = (hi - lo - 1) / 64 + 1, units = lo + lane * step;
+            const int b = 63 - __clzll(__ballot((above(units) > at) & (units < hi)));
+            lo += b * step;
+            hi = min(hi, lo + step);
+        }
+        int r = at - __builtin_amdgcn_readfirstlane(above(lo + 1));
+        unsigned long long of = __ballot(lane < S && c.ahead <= lo && lo < c.ahead + c.tiles);
+        while (r-- > 0) of &= of - 1;
+        const int s = __ffsll(of) - 1;
+        tile = lo - of_lane(c.ahead, s);
+        return s;
+    }
+    __device__ __forceinline__ int parts(int units) const { return (units + part - 1) / part; }
+};
 
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2) void attend_chunk(AttendArgs a) {
@@ -411,20 +462,31 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
     const int group = p.Hq / p.Hkv, Dh = p.Dh;
     const int kvh = blockIdx.x % p.Hkv, tile_id = blockIdx.x / p.Hkv;
     // ---- rows of no stream are 0
-    if (kvh == 0 && blockIdx.y == 0) {
+    if (kvh == 0) {
         const int lo = min(max(p.offsets[0], 0), p.M), hi = min(max(p.offsets[p.S], 0), p.M), none = lo + p.M - hi;
         for (int r = tile_id; r < none; r += gridDim.x / p.Hkv) {
             T* o = (T*)a.out + (int64_t)(r < lo ? r : hi + r - lo) * p.Hq * Dh;
             for (int i = tid; i < p.Hq * Dh; i += NT) o[i] = (T)0.f;
         }
     }
-    // ---- stream and rows of this block
-    int s = -1, row0 = 0, n_rows = 0, start = 0;
-    if (p.S <= LONGEST_FIRST) {
+    // ---- stream and rows of this block, and which part of their keys: first the parts beyond the first of long row tiles, then all
+    // row tiles, the longest first
+    int s = -1, row0 = 0, n_rows = 0, start = 0, n_parts = 1, my_part = 0, slot = 0;
+    if (p.S <= CHUNK_STREAMS) {
         const ChunkStream c(p, lane);
+        const ChunkPlan plan(c, p.S, p.Hkv, a.extra, chunk_least<T>() * group / R + 1, chunk_start<T>() * group / R);
+        int at;
+        if (tile_id < plan.beyond()) {
+            my_part = plan.part_of(tile_id, at);
+            slot = plan.cut() + tile_id;                // of the pieces: the first parts of the cut tiles, then the others
+        } else {
+            slot = at = tile_id - plan.beyond();
+            if (at >= plan.tiles()) return;
+        }
         int tile;
-        s = longest_first(c, p.S, tile_id, tile);
-        if (s >= 0) { start = of_lane(c.start, s); n_rows = of_lane(c.rows, s) * group; row0 = tile * R; }
+        s = plan.find(at, tile);
+        start = of_lane(c.start, s); n_rows = of_lane(c.rows, s) * group; row0 = tile * R;
+        n_parts = plan.parts(of_lane(c.ahead, s) + tile + 1);
     } else {                                                                // the streams end to end, a stream's last (longest) tile first
         int64_t before = 0;
         for (int b = 0; b < p.S && s < 0; b += 64) {
@@ -450,9 +512,9 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
     const int pos = at(tok);                                                // this lane's row sees keys up to here
     const int b_lo = at(row0 / group), b_hi = at((min(row0 + R, n_rows) - 1) / group);
     int t_lo = 0, t_hi = b_hi < 0 ? 0 : (int)((paged_keys(p.width, p.page_shift, b_hi) - 1) / KT) + 1;
-    if (a.splits > 1) {
-        const int per = (t_hi + a.splits - 1) / a.splits;
-        t_lo = min(t_hi, (int)blockIdx.y * per); t_hi = min(t_hi, t_lo + per);
+    if (n_parts > 1) {
+        const int per = (t_hi + n_parts - 1) / n_parts;
+        t_lo = min(t_hi, my_part * per); t_hi = min(t_hi, t_lo + per);
     }
     // ---- Q fragments
     u32x4 qf[TL::CPR / 2];
@@ -671,17 +733,19 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
     }
     for (; t < t_hi; ++t) tile(t, std::false_type{});
     l += __shfl_xor(l, 32);
-    if (r >= n_rows) return;
-    const int64_t orow = (int64_t)(start + tok) * p.Hq + h;
-    if (a.splits > 1) {
-        float* o = a.part + ((int64_t)blockIdx.y * p.M * p.Hq + orow) * (DP + 2);
+    if (n_parts > 1) {
+        float* o = a.part + ((int64_t)slot * p.Hkv + kvh) * chunk_piece(DP);
+        const int row = wave * 32 + l31;
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
-            for (int c = 0; c < 16; ++c) o[i * 32 + 8 * (c >> 2) + 4 * hf + (c & 3)] = acc[i][c];
-        if (hf == 0) { o[DP] = m; o[DP + 1] = l; }
+            for (int c4 = 0; c4 < 4; ++c4)
+                *(f32x4*)(o + ((i * 8 + 2 * c4 + hf) * R + row) * 4) = f32x4{acc[i][4 * c4], acc[i][4 * c4 + 1], acc[i][4 * c4 + 2], acc[i][4 * c4 + 3]};
+        if (hf == 0) { o[DP * R + row] = m; o[(DP + 1) * R + row] = l; }
         return;
     }
+    if (r >= n_rows) return;
+    const int64_t orow = (int64_t)(start + tok) * p.Hq + h;
     const float inv = 1.f / l;
     T* o = (T*)a.out + orow * Dh;
 #pragma unroll
@@ -696,67 +760,55 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
         }
 }
 
-// Adds the parts of a row's keys.  One wave per row and head.
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attend_chunk_join(AttendArgs a) {
+// Adds the parts of the row tiles that were cut, in the order of the keys.  A block per place and 8 Q dims, a thread
+// per row and 4 Q: where there are few row tiles, finer (2 tiles in 31 parts: 16 blocks of 8 batches of loads otherwise).
+template <typename T, int DP, int Q>
+__global__ __launch_bounds__(2 * CHUNK_ROWS) void attend_chunk_join(AttendArgs a) {
+    constexpr int R = CHUNK_ROWS;
     const PagedArgs& p = a.p;
-    const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (orow >= (int64_t)p.M * p.Hq) return;
-    const int lane = threadIdx.x & 63;
-    // a lane's is one part (64 at most): their factors first, so that their rows are requested side by side
-    const float* first = a.part + orow * (DP + 2);
-    const int64_t step = (int64_t)p.M * p.Hq * (DP + 2);
-    const float* mine = first + min(lane, a.splits - 1) * step;
-    const float m = mine[DP], l = mine[DP + 1];                 // (rows of no stream: whatever is there, unused)
-    int pos;
-    const int s = paged_row(p, (int)(orow / p.Hq), pos);
-    T* out = (T*)a.out + orow * p.Dh;
-    if (s >= p.S || pos < 0) {
-        for (int d = lane; d < p.Dh; d += 64) out[d] = (T)0.f;
-        return;
+    const int group = p.Hq / p.Hkv, lane = threadIdx.x & 63, kvh = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    const ChunkStream c(p, lane);
+    const ChunkPlan plan(c, p.S, p.Hkv, a.extra, chunk_least<T>() * group / R + 1, chunk_start<T>() * group / R);
+    if (at >= plan.cut()) return;
+    int tile;
+    const int s = plan.find(at, tile), start = of_lane(c.start, s), n_rows = of_lane(c.rows, s) * group, parts = plan.parts(of_lane(c.ahead, s) + tile + 1);
+    __shared__ int place[CHUNK_LEVELS];
+    if (threadIdx.x < 64) place[lane] = lane ? plan.cut() + plan.upto - plan.level + at : at;
+    __syncthreads();
+    const int row = threadIdx.x % R, d4 = (blockIdx.y * 2 + threadIdx.x / R) * Q, r = tile * R + row;
+    if (r >= n_rows || d4 * 4 >= p.Dh) return;
+    auto piece_of = [&](int j) { return a.part + ((int64_t)place[j] * p.Hkv + kvh) * chunk_piece(DP); };
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < parts; ++j) M = fmaxf(M, piece_of(j)[DP * R + row]);
+    const float MS = M == -INFINITY ? 0.f : M;
+    f32x4 acc[Q] = {};
+#pragma unroll 8 / Q
+    for (int j = 0; j < parts; ++j) {
+        const float* o = piece_of(j);
+        const float f = exp2_hw(o[DP * R + row] - MS);
+        L += o[(DP + 1) * R + row] * f;
+#pragma unroll
+        for (int k = 0; k < Q; ++k) acc[k] += *(const f32x4*)(o + ((d4 + k) * R + row) * 4) * f;
     }
-    float M = m;
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float factor = lane < a.splits ? exp2_hw(m - (M == -INFINITY ? 0.f : M)) : 0.f;
-    float L = lane < a.splits ? l * factor : 0.f, acc[(DP + 63) / 64];
-    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
+    const int tok = r / group, pos = paged_position(p.lengths[s], tok);
+    T* out = (T*)a.out + ((int64_t)(start + tok) * p.Hq + kvh * group + r - tok * group) * p.Dh + d4 * 4;
 #pragma unroll
-    for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = 0.f;
-    constexpr int U = 4;
-    for (int i = 0; i < a.splits; i += U) {
-        float x[U][(DP + 63) / 64];
+    for (int k = 0; k < Q; ++k) {
+        typename Vec<T, 4>::type v;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < (DP + 63) / 64; ++k) x[u][k] = first[min(i + u, a.splits - 1) * step + lane + 64 * k];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float f = __shfl(factor, i + u);              // (i + u < 64 + U: past the last part it is not used)
-            if (i + u < a.splits)
-#pragma unroll
-                for (int k = 0; k < (DP + 63) / 64; ++k) acc[k] = fmaf(x[u][k], f, acc[k]);
-        }
+        for (int e = 0; e < 4; ++e) v[e] = (T)(pos < 0 ? 0.f : acc[k][e] / L);
+        if ((d4 + k) * 4 < p.Dh) *(typename Vec<T, 4>::type*)(out + k * 4) = v;
     }
-#pragma unroll
-    for (int k = 0; k < (DP + 63) / 64; ++k)
-        if (lane + 64 * k < p.Dh) out[lane + 64 * k] = (T)(acc[k] / L);
 }
 
 int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
 int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
-// Parts of a row's keys, by the table's width (the lengths are on the device): none once every CU has its two blocks (16 streams
-// of 512 tokens, fp32: 79 us, 103 in two parts), otherwise as many as come to that without beginning another round of blocks.  A
-// part costs a row (Dh + 2) floats written and read.  That is as much as 250 keys' 16-bit products: such parts have 256 keys at
-// least (64 tokens behind 2000, 8 heads on 2 x 128: 20 us, 25 with 512 keys), and a table of 1536 keys is not cut (2 streams of 512
-// tokens, 32 heads on 8 x 64: 16 us, 27 in two parts).  It is little next to fp32 products (a tile of 32 keys x 128 dims takes 4 us):
-// 64 keys, and two rounds of blocks, which even out streams of different lengths (510 tokens of 4 streams behind 1117 to 4080,
-// 8 heads on 2 x 64: 167 us, 183 with one round; behind 2000 each 109 and 102).
-int chunk_splits(const PagedArgs& p, int elem) {
-    const int64_t tiles = std::max<int64_t>(1, ((int64_t)p.M * (p.Hq / p.Hkv) + CHUNK_ROWS / 2) / CHUNK_ROWS), blocks = tiles * p.Hkv;
-    const int64_t keys = (int64_t)p.width << p.page_shift, least = elem == ELEM_F32 ? 64 : 256;
-    if (blocks >= 512 || (elem != ELEM_F32 && keys < 1536)) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(64, std::min(keys / least, (elem == ELEM_F32 ? 1024 : 512) / blocks)));
+// Parts beyond the first that all row tiles together may be cut into, by the table's width (the lengths are on the device)
+template <typename T> int chunk_extra(const PagedArgs& p) {
+    const int64_t keys = (int64_t)p.width << p.page_shift;
+    return p.S > CHUNK_STREAMS || keys < 6 * chunk_least<T>() ? 0 : CHUNK_EXTRA;
 }
 // A cache that cannot hold more than this is not worth a second launch: 8 streams of 100 or 500 tokens, 8 heads on 2 x 64, take 8.9 us
 // with a block per segment and 13 in shares, of 1000 tokens 12 both ways, of 4000 35 and 13.
@@ -779,13 +831,16 @@ template <typename T, int DP> void run_chunk(AttendArgs a, hipStream_t s) {
         if (hipFuncSetAttribute((const void*)attend_chunk<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return;
         if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    const dim3 grid((unsigned)(chunk_tiles(a.p) * a.p.Hkv), (unsigned)a.splits);
-    attend_chunk<T, DP><<<grid, 64 * CHUNK_WAVES, bytes, s>>>(a);
-    if (a.splits > 1) attend_chunk_join<T, DP><<<(unsigned)(((int64_t)a.p.M * a.p.Hq + 3) / 4), 256, 0, s>>>(a);
+    a.extra = chunk_extra<T>(a.p);
+    const int more = (a.extra + a.p.Hkv - 1) / a.p.Hkv;
+    attend_chunk<T, DP><<<(unsigned)((chunk_tiles(a.p) + more) * a.p.Hkv), 64 * CHUNK_WAVES, bytes, s>>>(a);
+    if (!a.extra) return;
+    const unsigned places = (unsigned)(std::min<int64_t>(more, chunk_tiles(a.p)) * a.p.Hkv);
+    if (places < 128) attend_chunk_join<T, DP, 1><<<dim3(places, DP / 8), 2 * CHUNK_ROWS, 0, s>>>(a);
+    else attend_chunk_join<T, DP, 4><<<dim3(places, DP / 32), 2 * CHUNK_ROWS, 0, s>>>(a);
 }
 template <typename T, int DP> void run(AttendArgs a, int elem, hipStream_t s) {
     if (!a.p.offsets) { run_one<T, DP>(a, s); return; }
-    a.splits = chunk_splits(a.p, elem);
     run_chunk<T, DP>(a, s);
 }
 template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s) {
@@ -801,8 +856,8 @@ template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s)
 int64_t attend_workspace(const AttendArgs& a, int elem) {
     const int DP = padded_dim(a.p.Dh);
     if (!a.p.offsets) return one_whole(a.p) ? 0 : (int64_t)ONE_GRID * 2 * piece_floats(DP) * (int64_t)sizeof(float);
-    const int n = chunk_splits(a.p, elem);
-    return n > 1 ? (int64_t)n * a.p.M * a.p.Hq * (DP + 2) * (int64_t)sizeof(float) : 0;
+    const int extra = elem == ELEM_F32 ? chunk_extra<float>(a.p) : chunk_extra<f16>(a.p), more = (extra + a.p.Hkv - 1) / a.p.Hkv;
+    return extra ? (int64_t)2 * more * a.p.Hkv * chunk_piece(DP) * (int64_t)sizeof(float) : 0;
 }
 void launch_attend(AttendArgs a, int elem, hipStream_t s) {
     if (elem == ELEM_F32) run_dim<float>(a, elem, s);
