@@ -334,10 +334,11 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // next tile requested at the start of a tile and stored at its end.  Inside a wave the exponentials of 16 keys run under the
 // matrix instructions of the 16 before them.  The blocks of a stream walk the keys side by side, so that L2 serves 93 % of what
 // they read; equal shares of all the work, cut anywhere, would lose that (51 %) and 25 % of the speed.
-// Bound by instruction issue: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
+// Bound by issue and waits: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
 // with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
-// 412 us, 790 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
-// 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.  Two row sets per wave, or three waves per SIMD, spill; 32 keys per tile: 430 us.
+// 418 us, 780 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
+// 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.
+// Two row sets per wave, or three waves per SIMD, spill; tiles of 32 keys, eight-wave blocks and staggered halves are slower.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
 
@@ -370,10 +371,13 @@ struct ChunkStream {
         ahead = (int)min((int64_t)1 << 29, min((int64_t)max(past, 0), (int64_t)p.width << p.page_shift) * group / CHUNK_ROWS);
     }
 };
-// The work of up to 64 streams: their row tiles by the keys they look at, the most first, and the long ones in parts.  A stream's
-// tile t has ahead + t + 1 units of keys; one of more than `part` units is cut, into level 0 .. of it.  Run by a whole wave, a lane a
-// stream; uniform results, which depend on the lengths alone.
-constexpr int CHUNK_STREAMS = 64, CHUNK_LEVELS = 64, CHUNK_SLOTS = 512;
+// The work of up to 32 streams: their row tiles by the keys they look at, the most first, and the long ones in parts.  A stream's
+// tile t has ahead + t + 1 units of keys; one of more than `part` units is cut.  Run by a whole wave, a lane a stream; uniform
+// results, which depend on the lengths alone and are exact in every kernel (whole numbers and halves below 2^53).
+// 4 x 510 tokens behind 1117 to 4080, 8 heads on 2 x 64, fp32: 133 us, 154 with every row tile in the same number of parts.  12 streams
+// of 200 to 900 tokens behind up to 6000, 16 heads on 4 x 64, bf16: 70 to 113 us, 123 to 134 uncut.  It takes about 50 instructions per
+// stream, twice: 64 streams of 4 tokens behind 2000 would take 66 us with it and take 42 without.
+constexpr int CHUNK_STREAMS = 32, CHUNK_LEVELS = 64, CHUNK_SLOTS = 512;
 struct ChunkPlan {
     const ChunkStream& c;
     int S, part;
@@ -404,9 +408,11 @@ struct ChunkPlan {
             const double share = all / extra * (lane + 16) / 16;
             const int floor = max(least, (most + CHUNK_LEVELS - 1) / CHUNK_LEVELS);
             const unsigned mine = lane == 63 || share > most ? most : max(floor, (int)share + 1);
-            for (int s = 0; s < S; ++s) {       // of a stream, about: the shortest tile's and the longest's
+            const float inv = __builtin_amdgcn_rcpf((float)mine);
+            for (int s = 0; s < S; ++s) {       // of a stream, about: the shortest tile's and the longest's (1e-4: a whole number stays one)
                 const int t = of_lane(c.tiles, s), a = of_lane(c.ahead, s);
-                parts += 0.5 * t * ((a + t + mine - 1) / mine + (a + mine) / mine);
+                const float longest = ceilf(__builtin_fmaf((float)(a + t), inv, -1e-4f)), shortest = ceilf(__builtin_fmaf((float)(a + 1), inv, -1e-4f));
+                parts += 0.5 * t * (double)(longest + shortest);
             }
             parts *= Hkv;
             const double cost = parts <= CHUNK_SLOTS ? (double)mine + start : (all + parts * start) / CHUNK_SLOTS + 0.5 * mine;
@@ -805,7 +811,10 @@ __global__ __launch_bounds__(2 * CHUNK_ROWS) void attend_chunk_join(AttendArgs a
 int padded_dim(int Dh) { return Dh <= 64 ? 64 : Dh <= 128 ? 128 : 256; }
 
 int64_t chunk_tiles(const PagedArgs& p) { return (int64_t)p.M * (p.Hq / p.Hkv) / CHUNK_ROWS + p.S; }
-// Parts beyond the first that all row tiles together may be cut into, by the table's width (the lengths are on the device)
+// Parts beyond the first that all row tiles together may be cut into, by the table's width (the lengths are on the device).  A part
+// costs a row (Dh + 2) floats written and read: as much as 250 keys' 16-bit products, little next to fp32 ones (a tile of 32 keys x
+// 128 dims takes 4 us).  So parts have 256 or 64 keys at least (64 tokens behind 2000, 8 heads on 2 x 128, bf16: 20 us, 25 in parts of
+// 512), and a table of fewer than six is not cut at all (2 streams of 512 tokens, 32 heads on 8 x 64: 16 us, 27 in two parts).
 template <typename T> int chunk_extra(const PagedArgs& p) {
     const int64_t keys = (int64_t)p.width << p.page_shift;
     return p.S > CHUNK_STREAMS || keys < 6 * chunk_least<T>() ? 0 : CHUNK_EXTRA;

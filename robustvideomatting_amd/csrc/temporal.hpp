@@ -49,7 +49,7 @@ struct AttendArgs {
     const void *q, *k_pages, *v_pages; void* out;       // out [M][Hq][Dh]
     int64_t q_sm, q_sh;
     float scale_log2e;                                  // softmax runs in base 2
-    float* part; int splits, extra;
+    float* part; int splits, extra;                     // workspace; single tokens in shares; parts beyond the first of row tiles
 };
 int64_t attend_workspace(const AttendArgs& a, int elem);
 void launch_attend(AttendArgs a, int elem, hipStream_t s);
