@@ -460,6 +460,25 @@ def test_attend(dtype, lengths, new, Hq, Hkv, Dh, page):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("lengths,new,Hq,Hkv,Dh,page", [
+    ([6000], [4], 2, 2, 64, 64), ([3000, 0, 50, 2000, -20, 700], [5, 300, 0, 64, 40, 1], 6, 2, 80, 16), ([2500, 1600], [130, 33], 40, 40, 32, 32),
+    ([47 * i % 1700 - 40 for i in range(32)], [2] * 32, 4, 1, 64, 64), ([47 * i % 1700 - 40 for i in range(33)], [2] * 33, 4, 1, 64, 64),
+    ([1900, 4, 1900], [20, 700, 20], 8, 1, 200, 128), ([3000, 10, 900], [140, 140, 140], 300, 2, 16, 64),
+])
+def test_attend_chunks_in_parts(dtype, lengths, new, Hq, Hkv, Dh, page):
+    """Long keys behind few rows beside short ones: row tiles that are cut into parts, and others that are not."""
+    from robustvideomatting_amd import temporal as M
+    dt, g = DT[dtype], _gen(sum(new) + Dh)
+    cache, table, rows, lens = _attend_case(g, lengths, new, Hq, Hkv, Dh, page, dt, float("nan"))
+    off = _offsets(new)
+    q = _rn(g, off[-1], Hq, Dh, dtype=dt)
+    got = M.attend(q, cache, table, lens, torch.tensor(off, dtype=torch.int32).cuda())
+    ref, bound = O.attend(q, *cache, rows, lengths, off)
+    _near(got, ref, O.rounded(ref, bound, dt), "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("new", [[1, 1], [40, 3], [300, 17]])
 def test_attend_large_scores_and_scale(dtype, new):
     """Scores in the hundreds (weights of nearly 0 and 1), another scale than the default."""
