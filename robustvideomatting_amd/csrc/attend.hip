@@ -336,7 +336,7 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // they read; equal shares of all the work, cut anywhere, would lose that (51 %) and 25 % of the speed.
 // Bound by issue and waits: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
 // with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
-// 418 us, 780 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
+// 405 to 419 us, 790 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
 // 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.
 // Two row sets per wave, or three waves per SIMD, spill; tiles of 32 keys, eight-wave blocks and staggered halves are slower.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
