@@ -37,7 +37,7 @@ int paged_check(const char* who, PagedArgs& p, const int32_t* table, const int32
     if (pages < 1 || pages > INT_LIMIT || width < 1 || width > INT_LIMIT || width * page > INT_LIMIT + 1) return fail(who, "bad page pool or table");
     if (Hkv * page * Dh > INT_LIMIT / 4) return fail(who, "bad page pool or table: a page of all heads must stay below 2 GiB in fp32");
     // what the kernels launch for M rows of S streams: at most 256 threads a row, a tile of 128 rows, or a (stream, key head, 16 heads)
-    if (M * 256 > THREAD_LIMIT || M * Hq > INT_LIMIT / 2 || S * Hkv * ((Hq / Hkv + 15) / 16) * 256 > THREAD_LIMIT / 2) return fail(who, "too large for one launch");
+    if (M * 256 > THREAD_LIMIT || M * Hq > INT_LIMIT / 4 || S * Hkv * ((Hq / Hkv + 15) / 16) * 256 > THREAD_LIMIT / 2) return fail(who, "too large for one launch");
     if (M && S && (!table || !lengths)) return fail(who, "null table or lengths");
     memset(&p, 0, sizeof p);
     p.table = table; p.lengths = lengths; p.offsets = offsets;

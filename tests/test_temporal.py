@@ -117,6 +117,7 @@ def test_c_entries_refuse_bad_arguments_before_any_launch(entry, base, change, t
     ("rvm_attend", ATTEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
     ("rvm_attend", ATTEND_OK, dict(M=1 << 20, S=8, offsets=4096, Hq=4096), "too large"),
     ("rvm_attend", ATTEND_OK, dict(M=8, S=1 << 21, offsets=4096, Hq=8, Hkv=8), "too large"),
+    ("rvm_attend", ATTEND_OK, dict(M=1 << 21, S=1 << 20, offsets=4096, Hq=260, Hkv=4), "too large"),
     ("rvm_attend", ATTEND_OK, dict(M=1 << 20, S=1 << 20, Hq=1024), "too large"),
     ("rvm_attend", ATTEND_OK, dict(Hkv=8192, Hq=8192, page=1024, Dh=128), "below 2 GiB"),
     ("rvm_attend", ATTEND_OK, dict(width=64), "workspace"),
