@@ -133,11 +133,14 @@ def _dense_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _rows(t):
-    """[rows, heads, dim] in 16-byte pieces: as it is, or a dense copy."""
+def _rows(t, per):
+    """[rows, heads, dim] in 16-byte pieces (``per`` elements) - as it is, or a dense copy - its address and its two strides."""
     s0, s1, s2 = t.stride()
-    per = 16 // t.element_size()
-    return t if s2 == 1 and s0 % per == 0 and s1 % per == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    at = t.data_ptr()
+    if s2 == 1 and not (s0 % per or s1 % per or at % 16):
+        return t, at, s0, s1
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def _dense_like(t):
@@ -281,21 +284,21 @@ def append_kv(k, v, cache, table, lengths, offsets=None, freqs=None, q=None, int
         ok = False
     if not ok:
         _refuse_append(k, v, cache, table, lengths, offsets, freqs, q)
-    k, v = _rows(k), _rows(v)
-    rot = fp = qp = out_p = q_sm = q_sh = 0
+    per = 4 if dt is _F32 else 8
+    k, k_at, k_sm, k_sh = _rows(k, per)
+    v, v_at, v_sm, v_sh = _rows(v, per)
+    rot = fp = q_at = out_at = q_sm = q_sh = 0
     out = None
     if freqs is not None:
         freqs = freqs.contiguous()
         rot, fp = 2 * freqs.shape[0], freqs.data_ptr()
     if q is not None:
-        q = _rows(q)
+        q, q_at, q_sm, q_sh = _rows(q, per)
         out = _dense_like(q)
-        qp, out_p, (q_sm, q_sh, _) = q.data_ptr(), out.data_ptr(), q.stride()
-    k_sm, k_sh, _ = k.stride()
-    v_sm, v_sh, _ = v.stride()
+        out_at = out.data_ptr()
     S, width = table.shape
     _call(native.lib().rvm_append_kv, _DTYPES[dt],
-          _APPEND.pack(qp, k.data_ptr(), v.data_ptr(), out_p, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+          _APPEND.pack(q_at, k_at, v_at, out_at, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), lengths.data_ptr(),
                        0 if offsets is None else offsets.data_ptr(), fp, q_sm, q_sh, k_sm, k_sh, v_sm, v_sh,
                        M, S, qs[1], H, Dh, kp.shape[0], kp.shape[2], width, rot, bool(interleaved)), di)
     return out
@@ -334,12 +337,11 @@ def attend(q, cache, table, lengths, offsets=None, scale=None):
     S, width = table.shape
     code = _DTYPES[dt]
     need = _attend_workspace(code, offsets is not None, M, S, Hq, Hkv, Dh, P, page, width)
-    q = _rows(q)
+    q, q_at, sm, sh = _rows(q, 4 if dt is _F32 else 8)
     out = _dense_like(q)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    sm, sh, _ = q.stride()
     _call(native.lib().rvm_attend, code,
-          _ATTEND.pack(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, table.data_ptr(),
+          _ATTEND.pack(q_at, kp.data_ptr(), vp.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, table.data_ptr(),
                        lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), sm, sh, M, S, Hq, Hkv, Dh, P, page, width, need,
                        Dh ** -0.5 if scale is None else float(scale)), di)
     return out
