@@ -111,8 +111,9 @@ def rotate(x, pos, freqs, interleaved=False):
     return r, bound
 
 
-def attend(q, kp, vp, table, lengths, offsets=None, scale=None):
-    """Row by row from host copies of table, lengths and offsets.  Bad pages give NaN."""
+def attend(q, kp, vp, table, lengths, offsets=None, scale=None, parts=1):
+    """Row by row from host copies of table, lengths and offsets.  Bad pages give NaN.  `parts`: how many numbers of the
+    tensors' type a weight is multiplied as, for the bound."""
     M, Hq, Dh = q.shape
     P, Hkv, page, _ = kp.shape
     scale = Dh ** -0.5 if scale is None else scale
@@ -145,5 +146,7 @@ def attend(q, kp, vp, table, lengths, offsets=None, scale=None):
         if q.dtype != torch.float32:
             # weights are rounded to the tensors' type for the product with v, the largest of those seen so far being 1 or
             # more: half a step each, and below the smallest normal number half a step of that
-            bound[m] += away * half + v.abs().sum(1) * torch.finfo(q.dtype).tiny * half / l
+            # (in two parts: half a step of what the first half step left out, at least 2^7 times as fine at the low end, and twice as many products)
+            bound[m] += away * half ** parts + v.abs().sum(1) * torch.finfo(q.dtype).tiny * half / l / (1 if parts == 1 else 2 ** 7)
+            bound[m] += away * U * n * (parts - 1)
     return out, bound

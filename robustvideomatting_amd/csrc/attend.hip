@@ -61,15 +61,47 @@ template <typename T> __device__ __forceinline__ u32x4 piece_once(const T* p, bo
     return __builtin_nontemporal_load(ok ? (GlobalPiece)(uintptr_t)p : (GlobalPiece)(uintptr_t)&zero_piece);
 }
 
+// The matrix instruction takes weights of the tensors' type.  Each goes as two of them: rounded to it, and what that left out,
+// so that 2 x 8 or 2 x 11 digits of it count.
+template <typename T> struct TwoParts {
+    typedef typename Vec<T, 8>::type V8;
+    V8 upper, rest;
+    __device__ __forceinline__ void set(int i, float w) { upper[i] = (T)w; rest[i] = (T)(w - (float)upper[i]); }
+};
+// Whether some of the pieces hold an infinity or NaN: times 0 it is not 0.  (Times a remainder, which has any sign or is 0, an infinite
+// value is not what it is times the weight.)
+__device__ __forceinline__ float times0(f16 a, f16 b, float s) { typedef Vec<f16, 2>::type V2; return __builtin_amdgcn_fdot2(V2{a, b}, V2{0, 0}, s, false); }
+__device__ __forceinline__ float times0(bfl a, bfl b, float s) { typedef Vec<bfl, 2>::type V2; return __builtin_amdgcn_fdot2_f32_bf16(V2{a, b}, V2{0, 0}, s, false); }
+template <typename T, int N> __device__ __forceinline__ bool any_not_finite(const u32x4 (&v)[N]) {
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const auto x = __builtin_bit_cast(typename Vec<T, 8>::type, v[j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = times0(x[2 * k], x[2 * k + 1], s[k]);
+    }
+    return !((s[0] + s[1]) + (s[2] + s[3]) == 0.f);
+}
+template <typename V8> __device__ __forceinline__ V8 finite_only(V8 v) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (!__builtin_isfinite((float)v[k])) v[k] = 0;
+    return v;
+}
+
 // ---- one token per stream -------------------------------------------------------------------------------------------------
 // Work is cut by keys, not by streams: all streams' caches in units of NW tiles laid end to end, and block b of the grid
 // takes the b-th equal share, whatever the streams' lengths - they are known on the device only.  A (stream, key head, 16 query
 // heads) segment that fits inside a share is finished there; the pieces of one that does not go to the workspace (a block
 // has at most two such pieces: its first and its last) and attend_join adds them up in order.
-// Bound by memory: 8 streams of 8 to 65 thousand tokens, 8 key heads x 128 in bf16, 1.08 GB, take 170 us and 7 of joining, 6.4 TB/s
-// (a large copy reads and writes 5.2).  Keys and values are read past the caches: 193 us through them.
+// Bound by memory: 8 streams of 8 to 65 thousand tokens, 8 key heads x 128 in bf16, 1.08 GB, take 175 us and 7 of joining, 6.2 TB/s
+// (a large copy reads and writes 5.2).  Keys and values are read past the caches: 20 us more through them.  Weights in two parts cost
+// nothing beside the loads, looking for infinities 3 % (256 dims: 7).  With rounded weights the result is off by 2.2e-3 of its size
+// instead of the 1.7e-3 that one rounding to bf16 is (fp16: 2.5e-4, 2.1e-4).
 template <typename T> constexpr int one_kt() { return sizeof(T) == 2 ? 32 : 16; }         // keys per tile of a wave
 template <int DP> constexpr int one_nw() { return DP > 128 ? 2 : 4; }                      // waves of a block
+// fp16 weights are taken times 2^14, which the quotient does not see: below 2^-14 the type loses digits
+template <typename T> constexpr float one_lift() { return std::is_same<T, f16>::value ? 14.f : 0.f; }
 constexpr int ONE_ROWS = 16, ONE_GRID = 512;
 constexpr int piece_floats(int DP) { return ONE_ROWS * (DP + 2); }
 
@@ -192,6 +224,8 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
                 *(u32x4*)(kt_lds + (j * 64 + lane) * 16) = kr[j];
                 *(u32x4*)(vt_lds + (j * 64 + lane) * 16) = vr[j];
             }
+            bool odd = false;
+            if constexpr (sizeof(T) == 2) odd = __any(any_not_finite<T>(vr));
             if (t + NW < t_end) { load(t + NW); look(t + 2 * NW); }
             // ---- scores: lane = (row l15, keys 4 g .. 4 g + 3 of each 16)
             f32x4 sc[KT / 16];
@@ -218,7 +252,7 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
                 }
             mt = fmaxf(mt, __shfl_xor(mt, 16));
             mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn, al = exp2_hw(m - ms);
+            const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn, al = exp2_hw(m - ms), base = ms - one_lift<T>();
             m = mn;
             l *= al;
 #pragma unroll
@@ -226,16 +260,19 @@ __global__ __launch_bounds__(64 * one_nw<DP>(), DP > 128 ? 1 : 2) void attend_on
 #pragma unroll
             for (int kt = 0; kt < KT / 16; ++kt)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) { sc[kt][c] = exp2_hw(sc[kt][c] - ms); l += sc[kt][c]; }
+                for (int c = 0; c < 4; ++c) { sc[kt][c] = exp2_hw(sc[kt][c] - base); l += sc[kt][c]; }
             if constexpr (sizeof(T) == 2) {
-                typename Vec<T, 8>::type pf;                    // weights rounded to the tensors' type for the matrix instruction
+                TwoParts<T> w;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) { pf[c] = (T)sc[0][c]; pf[4 + c] = (T)sc[1][c]; }
+                for (int c = 0; c < 8; ++c) w.set(c, sc[c >> 2][c & 3]);
 #pragma unroll
                 for (int i = 0; i < DT; ++i) {
                     const int r = 4 * g + (l15 >> 2), c = 2 * i + ((l15 >> 1) & 1), o = (l15 & 1) * 8;
                     s16x4 v[2] = {read_tr(vt_lds + TL::template voff<16>(r, c) + o), read_tr(vt_lds + TL::template voff<16>(r + 16, c) + o)};
-                    acc[i] = mma16(__builtin_bit_cast(typename Vec<T, 8>::type, v), pf, acc[i]);
+                    auto vf = __builtin_bit_cast(typename Vec<T, 8>::type, v);
+                    acc[i] = mma16(vf, w.upper, acc[i]);
+                    if (odd) vf = finite_only(vf);
+                    acc[i] = mma16(vf, w.rest, acc[i]);
                 }
             } else {
 #pragma unroll
@@ -338,6 +375,8 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
 // 405 to 419 us, 790 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
 // 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.
+// 16-bit weights are rounded to the tensors' type for the product with the values: the result is off by 2.1e-3 of its size where one
+// rounding to bf16 is 1.7e-3 (fp16: 2.5e-4, 2.1e-4).  In two parts, as attend_one has them, the 5 streams take 540 us.
 // Two row sets per wave, or three waves per SIMD, spill; tiles of 32 keys, eight-wave blocks and staggered halves are slower.
 template <typename T> constexpr int chunk_kt() { return sizeof(T) == 2 ? 64 : 32; }       // keys per tile
 constexpr float LAZY = 8.f;         // the running maximum may lag by 2^8 before the sums are rescaled (weights up to 256: no loss)
@@ -695,7 +734,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, (int)sizeof(T) * DP > 256 ? 1 : 2
 #pragma unroll
             for (int c = 0; c < 8; ++c) w[c] = exp2_hw(fmaf(sc[k16 >> 1][(k16 & 1) * 8 + c], a.scale_log2e, -ms));
             if constexpr (sizeof(T) == 2) {
-                V8 pf;                                                      // rounded to the tensors' type for the matrix instruction
+                V8 pf;                                                      // (rounded)
 #pragma unroll
                 for (int c = 0; c < 8; ++c) pf[c] = (T)w[c];
 #pragma unroll

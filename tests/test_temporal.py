@@ -479,6 +479,48 @@ def test_attend_chunks_in_parts(dtype, lengths, new, Hq, Hkv, Dh, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("longest", [60, 3000])
+def test_attend_one_token_rounds_once(dtype, longest):
+    """One token a stream, 16-bit: the result is that of 32 bits, rounded once - the weights keep their digits."""
+    from robustvideomatting_amd import temporal as M
+    dt, g = DT[dtype], _gen(longest + 1)
+    for Hq, Hkv, Dh in ((8, 2, 64), (6, 3, 128), (2, 2, 256)):
+        lengths = [0, 1, 7, 31, 40, longest]
+        cache, table, rows, lens = _attend_case(g, lengths, [1] * 6, Hq, Hkv, Dh, 16, dt, float("nan"))
+        q = _rn(g, 6, Hq, Dh, dtype=dt)
+        got = M.attend(q, cache, table, lens)
+        ref, bound = O.attend(q, *cache, rows, lengths, parts=2)
+        _near(got, ref, O.rounded(ref, bound, dt), "out, heads of %d" % Dh)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_attend_one_token_with_values_that_are_not_finite(dtype, bad):
+    """A value that is not finite decides its own dim, for the heads that read it, and touches no other."""
+    from robustvideomatting_amd import temporal as M
+    dt, g, lengths = DT[dtype], _gen(17), [100, 20]
+    cache, table, rows, lens = _attend_case(g, lengths, [1, 1], 4, 2, 64, 16, dt, 0.0)
+    q = _rn(g, 2, 4, 64, dtype=dt)
+    clean, bound = O.attend(q, *cache, rows, lengths, parts=2 if dt != torch.float32 else 1)
+    for at, dim in ((0, 0), (37, 5), (100, 63)):
+        cell = cache[1][rows[0][at // 16], 1, at % 16]
+        keep = cell[dim].item()
+        cell[dim] = bad
+        got = M.attend(q, cache, table, lens)
+        cell[dim] = keep
+        want = clean.clone()
+        want[0, 2:, dim] = bad
+        hit = torch.zeros_like(want, dtype=torch.bool)
+        hit[0, 2:, dim] = True
+        assert torch.equal(got[hit].double().nan_to_num(7.0), want[hit].nan_to_num(7.0)), (at, got[hit])
+        got[hit] = 0
+        want[hit] = 0
+        _near(got, want, O.rounded(want, bound, dt), "out")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("new", [[1, 1], [40, 3], [300, 17]])
 def test_attend_large_scores_and_scale(dtype, new):
