@@ -1,10 +1,12 @@
 // Where a position of a stream lives in a paged cache.  Plain C++ on both sides, so that the bounds can be checked on the host.
 #pragma once
 #include <stdint.h>
+#ifndef RVM_HD
 #ifdef __HIPCC__
 #define RVM_HD __host__ __device__ __forceinline__
 #else
 #define RVM_HD inline
+#endif
 #endif
 // Position of the i-th new token (i >= 0) of a stream of `length` tokens; past the last int, that int
 RVM_HD int paged_position(int length, int i) {

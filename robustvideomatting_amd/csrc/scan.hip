@@ -1,5 +1,6 @@
 // Causal convolution over time and selective state space scan, for chunks of steps and for single steps.
 #include "temporal.hpp"
+#include "scan_index.hpp"
 #include <algorithm>
 
 namespace {
@@ -117,7 +118,6 @@ template <typename T> void run_conv_v(const CausalConvArgs& a, int vec, hipStrea
 // composes them over the block (the decay over a chunk is exp(A sum delta)): every chunk's first state within its block, and
 // the block's last.  FROM composes the blocks in front of it, then runs its chunks from there.
 enum ScanMode { SCAN_WHOLE, SCAN_ENDS, SCAN_FROM };
-constexpr int SCAN_BATCH = 4;                           // steps requested ahead, half of them for many states: 4 spill (58 x 171 x 99, 64 states: 79 us, not 61)
 constexpr int SCAN_WAVES = 8;                           // waves of a block where the time axis is cut (16: two thirds slower at 1021 steps)
 template <int MODE> constexpr int scan_waves() { return MODE == SCAN_WHOLE ? 2 : SCAN_WAVES; }
 template <int PACK> struct Lane { typedef int64_t type; };      // a lane's place from the wave's scalar address: of its sequence, too
@@ -126,7 +126,8 @@ template <int NP> constexpr int scan_occupancy() { return NP <= 16 ? 4 : NP <= 3
 
 template <typename T, int NP, int PACK, int MODE>
 __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) void selective_scan(ScanArgs a) {
-    constexpr int TB = NP * PACK <= 16 ? SCAN_BATCH : SCAN_BATCH / 2, NV = MODE == SCAN_ENDS ? NP : 2 * NP, LD = (TB * PACK * NV + 63) / 64, W = scan_waves<MODE>();
+    constexpr bool ENDS = MODE == SCAN_ENDS;
+    constexpr int TB = scan_batch(NP, PACK), NV = scan_values(NP, ENDS), LD = scan_loads(NP, PACK, ENDS), W = scan_waves<MODE>();
     constexpr int BC = LD * 64, TAB = NP * 64;
     constexpr int LDS = MODE == SCAN_ENDS ? (W * (TAB + 64) > W * 2 * BC ? W * (TAB + 64) : W * 2 * BC) : MODE == SCAN_FROM ? W * 2 * BC + TAB : W * 2 * BC;
     __shared__ __attribute__((aligned(16))) float lds[LDS];
@@ -160,7 +161,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
     for (int j = 0; j < LD; ++j) {
         const int e = j * 64 + lane, v = e % NV, n = min(v % NP, a.N - 1), q = min(e / NV % PACK, last);
         const int64_t st = v < NP ? a.B_st : a.C_st;
-        bp[j] = (v < NP ? Bm + q * a.B_sb : Cm + q * a.C_sb) + (e / (NV * PACK)) * st + n;
+        bp[j] = (v < NP ? Bm + q * a.B_sb : Cm + q * a.C_sb) + scan_step_of(e, NP, PACK, ENDS) * st + n;
         b_inc[j] = TB * st;
     }
     auto at = [&](const char* row, lane_t o) -> T { return *(const T*)(row + o); };
@@ -182,7 +183,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
             }
 #pragma unroll
             for (int j = 0; j < LD; ++j) {
-                const int k = (j * 64 + lane) / (NV * PACK);
+                const int k = scan_step_of(j * 64 + lane, NP, PACK, ENDS);
                 br[j] = k < left ? *bp[j] : (T)0.f;
             }
         }

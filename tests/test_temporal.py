@@ -173,6 +173,30 @@ def test_page_lookup_stays_inside_the_table_and_the_pool(tmp_path):
     assert [at(1, p) for p in (48, 2 ** 31 - 1, -1, -16)] == [-1] * 4
 
 
+def _scan_index(tmp_path):
+    src = tmp_path / "scan_index.cpp"
+    src.write_text('#include "%s/robustvideomatting_amd/csrc/scan_index.hpp"\nextern "C" {\nint batch(int np, int pack) { return scan_batch(np, pack); }\n'
+                   'int values(int np, int ends) { return scan_values(np, ends); }\nint loads(int np, int pack, int ends) { return scan_loads(np, pack, ends); }\n'
+                   'int step_of(int e, int np, int pack, int ends) { return scan_step_of(e, np, pack, ends); }\n}\n' % ROOT)
+    lib = tmp_path / "scan_index.so"
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(lib), str(src)])
+    return ctypes.CDLL(str(lib))
+
+
+@pytest.mark.parametrize("states", [8, 16, 32, 64])
+@pytest.mark.parametrize("pack", [1, 2, 4])
+@pytest.mark.parametrize("ends", [0, 1])
+def test_scan_lanes_stay_inside_their_batch(tmp_path, states, pack, ends):
+    """What a wave requests of B and C: every value of the batch, each at its place, and no step behind the batch - also
+    where the batch has fewer values than the wave has lanes."""
+    f = _scan_index(tmp_path)
+    batch, values, loads = f.batch(states, pack), f.values(states, ends), f.loads(states, pack, ends)
+    assert (loads - 1) * 64 < batch * pack * values <= loads * 64
+    steps = [f.step_of(e, states, pack, ends) for e in range(loads * 64)]
+    assert steps[:batch * pack * values] == [k for k in range(batch) for _ in range(pack * values)]
+    assert 0 <= min(steps) and max(steps) == batch - 1
+
+
 # ---- convolution --------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
