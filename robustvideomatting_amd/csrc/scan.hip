@@ -142,7 +142,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
     const int64_t b = b0 + seq;
     const int d_own = dti * 64 + lane - seq * a.nD, d = min(d_own, a.nD - 1);
     const bool own = d_own < a.nD;
-    const int t0 = MODE == SCAN_WHOLE ? 0 : min(a.T, ch * a.chunk_len), t1 = MODE == SCAN_WHOLE ? a.T : min(a.T, t0 + a.chunk_len);
+    const int t0 = MODE == SCAN_WHOLE ? 0 : scan_first_step(a.T, a.chunk_len, ch), t1 = MODE == SCAN_WHOLE ? a.T : scan_end_step(a.T, a.chunk_len, t0);
     // a wave's rows are at scalar addresses plus 4 bytes times the lane; B and C are dealt over the lanes, each with a pointer of its own
     const char* x = (const char*)((const T*)a.x + b0 * a.x_sb + (int64_t)t0 * a.x_st);
     const char* dt = (const char*)((const T*)a.dt + b0 * a.dt_sb + (int64_t)t0 * a.dt_st);
@@ -380,8 +380,6 @@ int scan_pack(int B, int T, int D, int N) {
     if (D > 32 || N > 32 || (T < 64 ? B : (int64_t)B * (T / SCAN_MIN_STEPS)) < 4096) return 1;
     return D <= 16 && N <= 16 ? 4 : 2;
 }
-// steps of a chunk: whole batches of loads
-int64_t scan_chunk_len(int64_t T, int64_t chunks) { return ((T + chunks - 1) / chunks + SCAN_BATCH - 1) / SCAN_BATCH * SCAN_BATCH; }
 int scan_chunks(int B, int T, int D, int N) {
     const int pack = scan_pack(B, T, D, N);
     const int64_t waves = ((int64_t)B + pack - 1) / pack * ((D + 63) / 64), W = SCAN_WAVES;

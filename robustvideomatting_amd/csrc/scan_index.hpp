@@ -20,3 +20,11 @@ RVM_HD constexpr int scan_step_of(int e, int NP, int PACK, bool ends) {
     const int k = e / (scan_values(NP, ends) * PACK), last = scan_batch(NP, PACK) - 1;
     return k < last ? k : last;
 }
+// Steps of a chunk: whole batches of loads
+RVM_HD int64_t scan_chunk_len(int64_t T, int64_t chunks) { return ((T + chunks - 1) / chunks + SCAN_BATCH - 1) / SCAN_BATCH * SCAN_BATCH; }
+// First step of a chunk and the one behind its last (both T where it has none); T and the length are below 2^31, their sums are not
+RVM_HD int scan_first_step(int T, int chunk_len, int chunk) {
+    const int64_t t = (int64_t)chunk * chunk_len;
+    return t < T ? (int)t : T;
+}
+RVM_HD int scan_end_step(int T, int chunk_len, int first) { return T - first > chunk_len ? first + chunk_len : T; }

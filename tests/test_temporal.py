@@ -177,7 +177,9 @@ def _scan_index(tmp_path):
     src = tmp_path / "scan_index.cpp"
     src.write_text('#include "%s/robustvideomatting_amd/csrc/scan_index.hpp"\nextern "C" {\nint batch(int np, int pack) { return scan_batch(np, pack); }\n'
                    'int values(int np, int ends) { return scan_values(np, ends); }\nint loads(int np, int pack, int ends) { return scan_loads(np, pack, ends); }\n'
-                   'int step_of(int e, int np, int pack, int ends) { return scan_step_of(e, np, pack, ends); }\n}\n' % ROOT)
+                   'int step_of(int e, int np, int pack, int ends) { return scan_step_of(e, np, pack, ends); }\n'
+                   'long long chunk_len(long long t, long long n) { return scan_chunk_len(t, n); }\nint first(int t, int len, int ch) { return scan_first_step(t, len, ch); }\n'
+                   'int end(int t, int len, int first) { return scan_end_step(t, len, first); }\n}\n' % ROOT)
     lib = tmp_path / "scan_index.so"
     subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(lib), str(src)])
     return ctypes.CDLL(str(lib))
@@ -195,6 +197,26 @@ def test_scan_lanes_stay_inside_their_batch(tmp_path, states, pack, ends):
     steps = [f.step_of(e, states, pack, ends) for e in range(loads * 64)]
     assert steps[:batch * pack * values] == [k for k in range(batch) for _ in range(pack * values)]
     assert 0 <= min(steps) and max(steps) == batch - 1
+
+
+@pytest.mark.parametrize("T,D,N", [(40, 8, 16), (63, 8, 4), (1021, 333, 13), (8160, 960, 16), (2 ** 31 - 65, 1, 1), (2 ** 31 - 65, 64, 1),
+                                   (2 ** 31 - 16385, 33, 64), (2 ** 31 - 16383, 64, 8), (2 ** 31 - 65, 900, 1)])
+def test_scan_chunks_cover_every_step_once(tmp_path, T, D, N):
+    """The chunks that a length is cut into, up to the longest that the entry takes: end to end, from 0 to T."""
+    from robustvideomatting_amd import native
+    f = _scan_index(tmp_path)
+    f.chunk_len.restype = ctypes.c_longlong
+    f.chunk_len.argtypes = [ctypes.c_longlong] * 2
+    need = native.lib().rvm_selective_scan_workspace(1, T, D, N)
+    chunks = need // 4 // ((N + 1) * D) * 8 // 9                # a slot a chunk, and one for every eight
+    assert chunks >= 8 and chunks % 8 == 0 and chunks * 9 // 8 * (N + 1) * D * 4 == need
+    length, at = f.chunk_len(T, chunks), 0
+    assert 0 < length < 2 ** 31
+    for ch in range(chunks):
+        first, end = f.first(T, length, ch), f.end(T, length, f.first(T, length, ch))
+        assert first == at and first <= end <= T, ch
+        at = end
+    assert at == T
 
 
 # ---- convolution --------------------------------------------------------------------------------------------------------
