@@ -84,7 +84,8 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* c, void* hip_stream) {
     if (c->nN < 1 || c->nN > 64) return fail(who, "1 to 64 states per channel");
     if (!c->nB || !c->nD) return 0;
     if (!c->A || !c->state_out || (c->nT && (!c->x || !c->dt || !c->B || !c->C || !c->y))) return fail(who, "null buffer");
-    if (c->nB * ((c->nD + 63) / 64) > THREAD_LIMIT / 128) return fail(who, "too large for one launch");
+    // (a row's bytes are a lane's 32-bit offset)
+    if (c->nB * ((c->nD + 63) / 64) > THREAD_LIMIT / 128 || c->nD * (elem == ELEM_F32 ? 4 : 2) > THREAD_LIMIT + 1) return fail(who, "too large for one launch");
     if (c->state_in == c->state_out) return fail(who, "state_out must not alias state_in");
     const int64_t need = rvm_selective_scan_workspace(c->nB, c->nT, c->nD, c->nN);
     if (need > 0 && (!c->workspace || c->workspace_bytes < need)) return fail(who, "workspace too small (rvm_selective_scan_workspace)");

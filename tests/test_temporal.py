@@ -112,6 +112,7 @@ def test_c_entries_refuse_bad_arguments_before_any_launch(entry, base, change, t
     ("rvm_causal_conv", CONV_OK, dict(B=1 << 20, T=1 << 20), "too large"),
     ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 26), "too large"),
     ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 20, nD=1 << 20), "too large"),
+    ("rvm_selective_scan", SCAN_OK, dict(nD=(1 << 30) + 1, nN=1), "too large"),
     ("rvm_append_kv", APPEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
     ("rvm_append_kv", APPEND_OK, dict(Hkv=4096, Hq=4096, page=1024, Dh=256, pages=1), "below 2 GiB"),
     ("rvm_attend", ATTEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
