@@ -18,6 +18,13 @@ __device__ __forceinline__ float softplus_f(float v) {
     return fmaxf(v, 0.f) + fmaf(LN2, __builtin_amdgcn_logf(w), e - (w - 1.f));
 }
 
+// 4^x h + e: a state behind many steps at once.  Where they make it grow past what a factor holds, the state itself may still be in
+// range, zero or tiny as it was: two factors of 2^127 at most take any normal number past the range
+__device__ __forceinline__ float carried(float x, float h, float e) {
+    const float f = exp2_hw(fminf(x, 127.f));
+    return fmaf(f * h, f, e);
+}
+
 // ---- causal convolution: y[t] = act(bias + sum_w weight[w] xx[t + w]) with xx = the W-1 rows of the state, then x ----
 // A thread has VEC channels (16 bytes where the rows allow it) of RUN steps, taken four at a time with the next four requested ahead: the chip then
 // reads, computes and writes at the same time, where threads that request a whole run at once go through the three together.
@@ -209,7 +216,7 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             row[k] = (int64_t)min(wave + k * W, a.N - 1) * a.nD;
-            A2n[k] = a.A[row[k] + d] * LOG2E;
+            A2n[k] = a.A[row[k] + d] * (0.5f * LOG2E);
             hb[k] = first ? first[row[k] + d] : 0.f;
         }
         for (int j0 = 0; j0 < (int)blockIdx.y; j0 += U) {
@@ -225,19 +232,19 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
             for (int u = 0; u < U; ++u)
                 if (j0 + u < (int)blockIdx.y)
 #pragma unroll
-                    for (int k = 0; k < NB; ++k) hb[k] = fmaf(exp2_hw(st[u] * A2n[k]), hb[k], e[u][k]);
+                    for (int k = 0; k < NB; ++k) hb[k] = carried(st[u] * A2n[k], hb[k], e[u][k]);
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k)
             if (wave + k * W < NP) H[(wave + k * W) * 64 + lane] = hb[k];
-        const float before = a.steps[slot + d];
+        const float before = 0.5f * a.steps[slot + d];
 #pragma unroll
         for (int n = 0; n < NP; ++n) h[n] = a.carry[slot * a.N + (int64_t)min(n, a.N - 1) * a.nD + d];
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             A2[n] = n < a.N ? A2[n] * LOG2E : 0.f;
-            h[n] = n < a.N ? fmaf(exp2_hw(A2[n] * before), H[n * 64 + lane], h[n]) : 0.f;
+            h[n] = n < a.N ? carried(A2[n] * before, H[n * 64 + lane], h[n]) : 0.f;
         }
     } else {
         if (MODE == SCAN_WHOLE && first) {
@@ -308,12 +315,12 @@ __global__ __launch_bounds__((64 * scan_waves<MODE>()), scan_occupancy<NP>()) vo
         float* tot = a.totals + (b * gridDim.y + blockIdx.y) * (int64_t)a.nD * (a.N + 1) + d;
         const int64_t slot0 = (b * a.chunks + blockIdx.y * W) * (int64_t)a.nD;
         for (int n = wave; n < a.N; n += W) {
-            const float A2n = a.A[(int64_t)n * a.nD + d] * LOG2E;
+            const float A2n = a.A[(int64_t)n * a.nD + d] * (0.5f * LOG2E);
             float hb = 0.f;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 if (own) a.carry[(slot0 + (int64_t)w * a.nD) * a.N + (int64_t)n * a.nD + d] = hb;
-                hb = fmaf(exp2_hw(A2n * S[w * 64 + lane]), hb, lds[w * TAB + n * 64 + lane]);
+                hb = carried(A2n * S[w * 64 + lane], hb, lds[w * TAB + n * 64 + lane]);
             }
             if (own) tot[(int64_t)n * a.nD] = hb;
         }

@@ -375,6 +375,33 @@ def test_scan_large_and_tiny_step_sizes(T):
     _near(y, ry, O.rounded(ry, by, torch.float32), "y")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("sign,softplus", [(1.0, False), (-1.0, False), (1.0, True)])
+@pytest.mark.parametrize("B,D,N", [(1, 70, 4), (2, 33, 16), (1, 40, 40)])
+def test_scan_states_that_grow_past_a_factor_s_range(dtype, sign, softplus, B, D, N):
+    """A stream's steps multiply a state by e^145, more than fp32 holds: one that is zero stays zero until its first input,
+    and a tiny one becomes a large one, where the time axis is cut and where it is not."""
+    from robustvideomatting_amd import temporal as M
+    dt, g, T = DT[dtype], _gen(N), 100
+    x, Bm, Cm = torch.zeros((B, T, D), dtype=dt, device="cuda"), _rn(g, B, T, N, dtype=dt), _rn(g, B, T, N, dtype=dt)
+    x[:, 90:, :D // 2] = _rn(g, B, 10, D // 2, dtype=dt)
+    h0 = _rn(g, B, N, D) * 1e-35
+    h0[..., :D // 2] = 0
+    A = torch.full((N, D), 1.45 * sign, device="cuda")
+    A[1::2] *= -0.5                                         # beside states that decay
+    step = torch.full((B, T, D), sign * (0.5 if softplus else 1.0), dtype=dt, device="cuda")
+    bias = torch.full((D,), 0.04, device="cuda") if softplus else None
+    y, h = M.selective_scan(x, step, A, Bm, Cm, None, None, bias, h0, softplus=softplus)
+    (ry, rh), (by, bh) = O.selective_scan(x, step, A, Bm, Cm, None, None, bias, h0, softplus=softplus)
+    assert torch.isfinite(rh).all() and rh.abs().max() > 1e24 and not ry[:, :90, :D // 2].any()
+    _near(h, rh, bh + 1e-37, "state")
+    _near(y, ry, O.rounded(ry, by, dt), "y")
+    for t in range(T):                                      # step by step
+        y1, h0 = M.selective_scan(x[:, t:t + 1], step[:, t:t + 1], A, Bm[:, t:t + 1], Cm[:, t:t + 1], None, None, bias, h0, softplus=softplus)
+    _near(h0, rh, bh + 1e-37, "state, step by step")
+
+
 # ---- paged cache --------------------------------------------------------------------------------------------------------
 def _paged(g, lengths, new, Hkv, Dh, page, dt, spare=2, fill=0.0):
     """Pools whose pages are dealt out at random; a table with room; -> (cache, table tensor, table list, lengths tensor)"""
