@@ -174,8 +174,8 @@ int rvm_selective_scan(int dtype, const rvm_scan_args* args, void* hip_stream);
  * p % page.  New tokens are packed rows: offsets [S+1] gives every stream's rows (NULL: one row per stream, M == S), and its
  * i-th row has position lengths[s] + i (lengths: tokens BEFORE this call, for append and attend alike).  All three are
  * device int32, so a captured call follows the cache as it grows.  A negative position is no token: nothing is stored, its
- * attention is 0.  Rows behind the last stream's come out as 0.  A page number outside the pool, or a column past the table,
- * is never followed: append drops the token, and attention over it is NaN.
+ * attention is 0.  Rows behind the last stream's come out as 0; rows without any stream (S = 0) are refused.  A page number
+ * outside the pool, or a column past the table, is never followed: append drops the token, and attention over it is NaN.
  * page: a power of two, 16..1024.  Dh: a multiple of 8 up to 256.
  *
  * rvm_append_kv stores k and v [M,Hkv,Dh]; the first `rot` dims of k, and of q [M,Hq,Dh] into q_out where given, are rotated

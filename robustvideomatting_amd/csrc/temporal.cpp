@@ -31,6 +31,7 @@ int paged_check(const char* who, PagedArgs& p, const int32_t* table, const int32
                 int64_t Hq, int64_t Hkv, int64_t Dh, int64_t pages, int64_t page, int64_t width) {
     if (M < 0 || S < 0 || M > INT_LIMIT || S > INT_LIMIT) return fail(who, "bad number of rows or streams");
     if (!offsets && M != S) return fail(who, "without offsets every stream has one row");
+    if (M && !S) return fail(who, "rows for no stream");
     if (Hkv < 1 || Hq < 1 || Hq > 65535 || Hq % Hkv) return fail(who, "the query heads must be a multiple of the key heads");
     if (Dh < 8 || Dh > 256 || Dh % 8) return fail(who, "head size must be a multiple of 8, at most 256");
     if (page < 16 || page > 1024 || (page & (page - 1))) return fail(who, "page size must be a power of two from 16 to 1024");
@@ -38,7 +39,7 @@ int paged_check(const char* who, PagedArgs& p, const int32_t* table, const int32
     if (Hkv * page * Dh > INT_LIMIT / 4) return fail(who, "bad page pool or table: a page of all heads must stay below 2 GiB in fp32");
     // what the kernels launch for M rows of S streams: at most 256 threads a row, a tile of 128 rows, or a (stream, key head, 16 heads)
     if (M * 256 > THREAD_LIMIT || M * Hq > INT_LIMIT / 4 || S * Hkv * ((Hq / Hkv + 15) / 16) * 256 > THREAD_LIMIT / 2) return fail(who, "too large for one launch");
-    if (M && S && (!table || !lengths)) return fail(who, "null table or lengths");
+    if (M && (!table || !lengths)) return fail(who, "null table or lengths");
     memset(&p, 0, sizeof p);
     p.table = table; p.lengths = lengths; p.offsets = offsets;
     p.S = (int)S; p.M = (int)M; p.pages = (int)pages; p.width = (int)width; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.Dh = (int)Dh;
@@ -109,7 +110,7 @@ int rvm_append_kv(int dtype, const rvm_append_args* c, void* hip_stream) {
     AppendArgs a; memset(&a, 0, sizeof a);
     if (int rc = paged_check(who, a.p, c->table, c->lengths, c->offsets, c->M, c->S, c->Hq, c->Hkv, c->Dh, c->pages, c->page, c->width)) return rc;
     if (c->rot < 0 || c->rot > c->Dh || c->rot % 16) return fail(who, "rotated dims must be a multiple of 16, at most the head size");
-    if (!c->M || !c->S) return 0;
+    if (!c->M) return 0;
     if (!c->k || !c->v || !c->k_pages || !c->v_pages || (c->rot && !c->freqs) || (c->q != nullptr) != (c->q_out != nullptr)) return fail(who, "null buffer");
     const int64_t v = elem == ELEM_F32 ? 4 : 8;
     if (!aligned16(c->q) || !aligned16(c->k) || !aligned16(c->v) || !aligned16(c->q_out) || !aligned16(c->k_pages) || !aligned16(c->v_pages) ||
@@ -137,14 +138,14 @@ static int attend_prepare(const char* who, int dtype, const rvm_attend_args* c, 
 int64_t rvm_attend_workspace(int dtype, const rvm_attend_args* c) {
     AttendArgs a; int elem;
     if (attend_prepare("rvm_attend_workspace", dtype, c, a, elem)) return -1;
-    return a.p.M && a.p.S ? attend_workspace(a, elem) : 0;
+    return a.p.M ? attend_workspace(a, elem) : 0;
 }
 
 int rvm_attend(int dtype, const rvm_attend_args* c, void* hip_stream) {
     const char* who = "rvm_attend";
     AttendArgs a; int elem;
     if (int rc = attend_prepare(who, dtype, c, a, elem)) return rc;
-    if (!c->M || !c->S) return 0;
+    if (!c->M) return 0;
     if (!c->q || !c->k_pages || !c->v_pages || !c->out) return fail(who, "null buffer");
     const int64_t v = elem == ELEM_F32 ? 4 : 8;
     if (!aligned16(c->q) || !aligned16(c->k_pages) || !aligned16(c->v_pages) || !aligned16(c->out) || c->q_sm % v || c->q_sh % v)

@@ -134,6 +134,20 @@ def test_c_entries_refuse_what_no_launch_holds(entry, base, change, text):
     _refused(getattr(native.lib(), entry)(0, block, None), text)
 
 
+@pytest.mark.parametrize("entry,base", [("rvm_append_kv", APPEND_OK), ("rvm_attend", ATTEND_OK)])
+def test_c_entries_refuse_rows_for_no_stream(entry, base):
+    """No stream, but rows: refused rather than left as they were.  Neither rows nor streams: nothing to do."""
+    import struct
+    from robustvideomatting_amd import native
+    pack = lambda v: struct.pack("%dqd" % (len(v) - 1) if "scale" in v else "%dq" % len(v), *v.values())
+    rows = pack(dict(base, S=0, offsets=4096))
+    _refused(getattr(native.lib(), entry)(0, rows, None), "no stream")
+    if entry == "rvm_attend":
+        assert native.lib().rvm_attend_workspace(0, rows) == -1
+    assert getattr(native.lib(), entry)(0, pack(dict(base, S=0, M=0)), None) == 0
+    assert getattr(native.lib(), entry)(0, pack(dict(base, S=2, M=0, offsets=4096)), None) == 0
+
+
 def test_positions_and_keys_stay_inside_an_int(tmp_path):
     """A stream's positions saturate instead of wrapping round, and a pass over its keys ends one behind the table."""
     src = tmp_path / "pos.cpp"
