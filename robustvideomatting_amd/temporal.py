@@ -11,12 +11,13 @@ what T calls with one step give.
 
 Everything is channels-last.  Tensors are fp32, fp16 or bf16 on one HIP device; sums, states and softmax statistics are
 fp32.  Work goes to the current stream of the tensors' device, nothing synchronises, every call can be captured into a HIP
-graph.  Inference only, like the network: tensors that need a gradient are refused.  No CPU fallback.
+graph.  Inference only, like the network: tensors that need a gradient or carry a tangent are refused.  No CPU fallback.
 """
 import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import native
 
@@ -40,6 +41,13 @@ def _tensor(what, t, dtype, dev, shape):
         raise RuntimeError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple("any" if b < 0 else b for b in shape)))
     if t.requires_grad and _grad():
         raise RuntimeError("%s needs a gradient: the temporal operators are inference only" % what)
+    if _forward._current_level >= 0 and _dual(t):
+        raise RuntimeError("%s carries a tangent: the temporal operators are inference only" % what)
+
+
+def _dual(*tensors):
+    """Whether one of them carries a tangent.  (To be asked inside a dual level only; no_grad does not end forward mode.)"""
+    return torch._C._is_fwd_grad_enabled() and any(t is not None and _forward.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _lead(what, t):
@@ -125,7 +133,8 @@ def _fits(rows, dt, di, kp, vp, table, lengths, offsets):
             lengths.shape == (S,) and table.get_device() == di and lengths.get_device() == di and table.is_contiguous() and
             lengths.is_contiguous() and (S or not M) and
             (M == S if offsets is None else offsets.dtype is _I32 and offsets.shape == (S + 1,) and offsets.get_device() == di and offsets.is_contiguous()) and
-            not ((rows.requires_grad or kp.requires_grad or vp.requires_grad) and _grad()))
+            not ((rows.requires_grad or kp.requires_grad or vp.requires_grad) and _grad()) and
+            not (_forward._current_level >= 0 and _dual(rows, kp, vp)))
 
 
 def _dense_last(t):
@@ -174,7 +183,8 @@ def causal_conv(x, weight, bias=None, state=None, silu=True):
               (bias is None or (bias.dtype is dt and bias.shape == (D,) and bias.get_device() == di)) and
               (state is None or (state.dtype is dt and state.shape == (B, W - 1, D) and state.get_device() == di)) and
               not (_grad() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-                                (state is not None and state.requires_grad))))
+                                (state is not None and state.requires_grad))) and
+              not (_forward._current_level >= 0 and _dual(x, weight, bias, state)))
     except (AttributeError, ValueError, IndexError):
         ok = False
     if not ok:
@@ -225,7 +235,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
               (z is None or (z.dtype is ty and z.shape == xs and z.get_device() == di)) and
               (dt_bias is None or (dt_bias.dtype is _F32 and dt_bias.shape == (nd,) and dt_bias.get_device() == di)) and
               (state is None or (state.dtype is _F32 and state.shape == (nb, N, nd) and state.get_device() == di)) and
-              not (_grad() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, state))))
+              not (_grad() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, state))) and
+              not (_forward._current_level >= 0 and _dual(x, dt, A, B, C, D, z, dt_bias, state)))
     except (AttributeError, ValueError, IndexError):
         ok = False
     if not ok:
@@ -279,7 +290,8 @@ def append_kv(k, v, cache, table, lengths, offsets=None, freqs=None, q=None, int
         ok = (dt in _DTYPES and _fits(k, dt, di, kp, vp, table, lengths, offsets) and kp.shape[1] == H and v.dtype is dt and v.shape == ks and
               v.get_device() == di and (q is None or (q.dtype is dt and qs == (M, qs[1], Dh) and q.get_device() == di)) and
               (freqs is None or (freqs.dtype is _F32 and freqs.dim() == 1 and freqs.get_device() == di)) and
-              not (_grad() and (v.requires_grad or (q is not None and q.requires_grad) or (freqs is not None and freqs.requires_grad))))
+              not (_grad() and (v.requires_grad or (q is not None and q.requires_grad) or (freqs is not None and freqs.requires_grad))) and
+              not (_forward._current_level >= 0 and _dual(v, q, freqs)))
     except (AttributeError, ValueError, IndexError, TypeError):
         ok = False
     if not ok:

@@ -47,6 +47,23 @@ def test_cpu_tensors_are_refused():
         M.attend(torch.zeros(1, 1, 8), (pages, pages), i[:, None], i)
 
 
+def test_tangents_are_refused():
+    """Forward mode's dual tensors, which need no gradient: their tangents would be lost, under no_grad too."""
+    import torch.autograd.forward_ad as F
+    from robustvideomatting_amd import temporal as M
+    x = torch.ones(2, 3)
+    with F.dual_level():
+        d = F.make_dual(x, x)
+        M._tensor("x", x, x.dtype, x.device, (2, -1))
+        assert not d.requires_grad and M._dual(None, x, d) and not M._dual(None, x)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="x carries a tangent"):
+                M._tensor("x", d, x.dtype, x.device, (2, -1))
+        with torch.inference_mode():
+            M._tensor("x", d, x.dtype, x.device, (2, -1))
+    M._tensor("x", x, x.dtype, x.device, (2, -1))
+
+
 def _refused(rc, text):
     from robustvideomatting_amd import native
     assert rc != 0 and text in native.lib().rvm_last_error().decode(), (rc, native.lib().rvm_last_error())
@@ -895,6 +912,27 @@ def test_refusals_on_the_device():
         M.attend(k, (pages[:, :, :8].contiguous(), pages[:, :, :8].contiguous()), t, t[:, 0].contiguous())
     with pytest.raises(native_error(), match="rotated"):
         M.append_kv(k, k, (pages, pages), t, t[:, 0].contiguous(), freqs=torch.zeros(4, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused_on_the_device():
+    """Each tensor argument of each operator in turn."""
+    import torch.autograd.forward_ad as F
+    from robustvideomatting_amd import temporal as M
+    z = lambda *shape: torch.zeros(shape, device="cuda")
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
+    conv = dict(x=z(1, 2, 8), weight=z(4, 8), bias=z(8), state=z(1, 3, 8))
+    scan = dict(x=z(1, 2, 8), dt=z(1, 2, 8), A=z(4, 8), B=z(1, 2, 4), C=z(1, 2, 4), D=z(8), z=z(1, 2, 8), dt_bias=z(8), state=z(1, 4, 8))
+    append = dict(k=z(2, 1, 16), v=z(2, 1, 16), kp=z(2, 1, 16, 16), vp=z(2, 1, 16, 16), freqs=z(8), q=z(2, 1, 16))
+    attend = dict(q=z(2, 1, 16), kp=z(2, 1, 16, 16), vp=z(2, 1, 16, 16))
+    paged = lambda f: lambda kp, vp, **a: f(cache=(kp, vp), table=torch.tensor([[0], [1]], dtype=torch.int32, device="cuda"), lengths=i(2), **a)
+    for call, args in ((M.causal_conv, conv), (M.selective_scan, scan), (paged(M.append_kv), append), (paged(M.attend), attend)):
+        call(**args)
+        with F.dual_level():
+            call(**args)
+            for name in args:
+                with pytest.raises(RuntimeError, match="carries a tangent"):
+                    call(**dict(args, **{name: F.make_dual(args[name], torch.ones_like(args[name]))}))
 
 
 def native_error():
