@@ -129,9 +129,10 @@ static int attend_prepare(const char* who, int dtype, const rvm_attend_args* c, 
     if (elem < 0) return fail(who, "bad dtype");
     memset(&a, 0, sizeof a);
     if (int rc = paged_check(who, a.p, c->table, c->lengths, c->offsets, c->M, c->S, c->Hq, c->Hkv, c->Dh, c->pages, c->page, c->width)) return rc;
-    if (!(c->scale > 0.0) || !std::isfinite(c->scale)) return fail(who, "scale must be positive and finite");
+    const float scale = (float)(c->scale * 1.4426950408889634);
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(who, "scale must be positive and finite in fp32");
     a.q = c->q; a.k_pages = c->k_pages; a.v_pages = c->v_pages; a.out = c->out; a.q_sm = c->q_sm; a.q_sh = c->q_sh;
-    a.scale_log2e = (float)(c->scale * 1.4426950408889634);
+    a.scale_log2e = scale;
     return 0;
 }
 

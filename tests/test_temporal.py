@@ -129,7 +129,6 @@ def test_c_entries_refuse_bad_arguments_before_any_launch(entry, base, change, t
     ("rvm_causal_conv", CONV_OK, dict(B=1 << 20, T=1 << 20), "too large"),
     ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 26), "too large"),
     ("rvm_selective_scan", SCAN_OK, dict(nB=1 << 20, nD=1 << 20), "too large"),
-    ("rvm_selective_scan", SCAN_OK, dict(nD=(1 << 30) + 1, nN=1), "too large"),
     ("rvm_append_kv", APPEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
     ("rvm_append_kv", APPEND_OK, dict(Hkv=4096, Hq=4096, page=1024, Dh=256, pages=1), "below 2 GiB"),
     ("rvm_attend", ATTEND_OK, dict(M=1 << 24, S=1 << 24), "too large"),
@@ -149,6 +148,23 @@ def test_c_entries_refuse_what_no_launch_holds(entry, base, change, text):
     assert set(v) == set(base)
     block = struct.pack("%dqd" % (len(v) - 1) if "scale" in v else "%dq" % len(v), *v.values())
     _refused(getattr(native.lib(), entry)(0, block, None), text)
+
+
+def test_scan_rows_past_32_bit_offsets_are_refused():
+    """fp32 rows of more than 4 GiB."""
+    import struct
+    from robustvideomatting_amd import native
+    v = dict(SCAN_OK, nD=(1 << 30) + 1, nN=1)
+    _refused(native.lib().rvm_selective_scan(0, struct.pack("%dq" % len(v), *v.values()), None), "too large")
+
+
+@pytest.mark.parametrize("scale", [3e38, 1e39, 1e300, float("inf"), 1e-46, 1e-300, -1e-50])
+def test_scales_outside_fp32_are_refused(scale):
+    """The kernels scale in fp32 (and in base 2): infinite there, or 0, which a masked score would turn into NaN."""
+    import struct
+    from robustvideomatting_amd import native
+    v = dict(ATTEND_OK, scale=scale)
+    _refused(native.lib().rvm_attend(0, struct.pack("%dqd" % (len(v) - 1), *v.values()), None), "scale")
 
 
 @pytest.mark.parametrize("entry,base", [("rvm_append_kv", APPEND_OK), ("rvm_attend", ATTEND_OK)])
