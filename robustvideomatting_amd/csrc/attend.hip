@@ -887,15 +887,14 @@ template <typename T, int DP> void run_chunk(AttendArgs a, hipStream_t s) {
     if (places < 128) attend_chunk_join<T, DP, 1><<<dim3(places, DP / 8), 2 * CHUNK_ROWS, 0, s>>>(a);
     else attend_chunk_join<T, DP, 4><<<dim3(places, DP / 32), 2 * CHUNK_ROWS, 0, s>>>(a);
 }
-template <typename T, int DP> void run(AttendArgs a, int elem, hipStream_t s) {
-    if (!a.p.offsets) { run_one<T, DP>(a, s); return; }
-    run_chunk<T, DP>(a, s);
+template <typename T, int DP> void run(const AttendArgs& a, hipStream_t s) {
+    if (!a.p.offsets) run_one<T, DP>(a, s); else run_chunk<T, DP>(a, s);
 }
-template <typename T> void run_dim(const AttendArgs& a, int elem, hipStream_t s) {
+template <typename T> void run_dim(const AttendArgs& a, hipStream_t s) {
     switch (padded_dim(a.p.Dh)) {
-        case 64: run<T, 64>(a, elem, s); break;
-        case 128: run<T, 128>(a, elem, s); break;
-        default: run<T, 256>(a, elem, s);
+        case 64: run<T, 64>(a, s); break;
+        case 128: run<T, 128>(a, s); break;
+        default: run<T, 256>(a, s);
     }
 }
 
@@ -908,7 +907,7 @@ int64_t attend_workspace(const AttendArgs& a, int elem) {
     return extra ? (int64_t)2 * more * a.p.Hkv * chunk_piece(DP) * (int64_t)sizeof(float) : 0;
 }
 void launch_attend(AttendArgs a, int elem, hipStream_t s) {
-    if (elem == ELEM_F32) run_dim<float>(a, elem, s);
-    else if (elem == ELEM_F16) run_dim<f16>(a, elem, s);
-    else run_dim<bfl>(a, elem, s);
+    if (elem == ELEM_F32) run_dim<float>(a, s);
+    else if (elem == ELEM_F16) run_dim<f16>(a, s);
+    else run_dim<bfl>(a, s);
 }
