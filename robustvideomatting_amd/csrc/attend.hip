@@ -94,9 +94,9 @@ template <typename V8> __device__ __forceinline__ V8 finite_only(V8 v) {
 // takes the b-th equal share, whatever the streams' lengths - they are known on the device only.  A (stream, key head, 16 query
 // heads) segment that fits inside a share is finished there; the pieces of one that does not go to the workspace (a block
 // has at most two such pieces: its first and its last) and attend_join adds them up in order.
-// Bound by memory: 8 streams of 8 to 65 thousand tokens, 8 key heads x 128 in bf16, 1.08 GB, take 175 us and 7 of joining, 6.2 TB/s
+// Bound by memory: 8 streams of 8 to 65 thousand tokens, 8 key heads x 128 in bf16, 1.08 GB, take 178 us and 7 of joining, 6.1 TB/s
 // (a large copy reads and writes 5.2).  Keys and values are read past the caches: 20 us more through them.  Weights in two parts cost
-// nothing beside the loads, looking for infinities 3 % (256 dims: 7).  With rounded weights the result is off by 2.2e-3 of its size
+// nothing beside the loads, looking for infinities 3 % (256 dims: 7).  fp32, 1.85 GB: 298 us.  With rounded weights the result is off by 2.2e-3 of its size
 // instead of the 1.7e-3 that one rounding to bf16 is (fp16: 2.5e-4, 2.1e-4).
 template <typename T> constexpr int one_kt() { return sizeof(T) == 2 ? 32 : 16; }         // keys per tile of a wave
 template <int DP> constexpr int one_nw() { return DP > 128 ? 2 : 4; }                      // waves of a block
@@ -371,9 +371,11 @@ __global__ __launch_bounds__(DP) void attend_join(AttendArgs a, int keys) {
 // next tile requested at the start of a tile and stored at its end.  Inside a wave the exponentials of 16 keys run under the
 // matrix instructions of the 16 before them.  The blocks of a stream walk the keys side by side, so that L2 serves 93 % of what
 // they read; equal shares of all the work, cut anywhere, would lose that (51 %) and 25 % of the speed.
-// Bound by issue and waits: a tile of 64 keys x 128 dims keeps the matrix pipe of a SIMD busy for 2048 cycles and its issue port,
-// with the exponentials, conversions and sums of two waves, for about 2800.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
-// 405 to 419 us, 790 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
+// Bound by the order of work inside a wave: a tile of 64 keys x 128 dims takes the two waves of a SIMD about 5600 cycles, of which they
+// keep its matrix pipe busy for 2048 (36 %) and its vector pipe for 44 %.  A wave issues for 40 % of its time, waits for its turn to issue
+// for 32 % and for data and the barrier for 28 %: its scores, their maximum and the first weights stand in a line in front of the
+// products with the values, and one other wave is too little to run under them.  5 streams of 100 to 8160 tokens, 16 heads on 4, bf16:
+// 408 us, 800 TF (a large matrix product reaches 1224 TF); 16 streams of 512 tokens behind 4080, 8 heads on 2 x 64, fp32: 640 us,
 // 114 TF (154): 96 % of the matrix rate inside the tiles, the rest goes into the start and end of blocks.
 // 16-bit weights are rounded to the tensors' type for the product with the values: the result is off by 2.1e-3 of its size where one
 // rounding to bf16 is 1.7e-3 (fp16: 2.5e-4, 2.1e-4).  In two parts, as attend_one has them, the 5 streams take 540 us.
@@ -415,7 +417,9 @@ struct ChunkStream {
 // results, which depend on the lengths alone and are exact in every kernel (whole numbers and halves below 2^53).
 // 4 x 510 tokens behind 1117 to 4080, 8 heads on 2 x 64, fp32: 133 us, 154 with every row tile in the same number of parts.  12 streams
 // of 200 to 900 tokens behind up to 6000, 16 heads on 4 x 64, bf16: 70 to 113 us, 123 to 134 uncut.  It takes about 50 instructions per
-// stream, twice: 64 streams of 4 tokens behind 2000 would take 66 us with it and take 42 without.
+// stream, twice: 64 streams of 4 tokens behind 2000, 8 heads on 2 x 64, fp16, would take 66 us with it and take 41 without.  More streams
+// than 32 are not cut, which costs them dear where one is long: 4 tokens each, one stream behind 60000 and the others behind 500, bf16,
+// take 61 us with 32 streams and 1032 with 33.
 constexpr int CHUNK_STREAMS = 32, CHUNK_LEVELS = 64, CHUNK_SLOTS = 512;
 struct ChunkPlan {
     const ChunkStream& c;

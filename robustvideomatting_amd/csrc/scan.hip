@@ -118,11 +118,11 @@ template <typename T> void run_conv_v(const CausalConvArgs& a, int vec, hipStrea
 // requested before the present ones are worked on.  Where there are half or fewer channels than lanes, a wave has those of PACK
 // sequences, whose B and C lie side by side in LDS.
 // Bound by instructions, the exponential costing two of the others (8 cycles a wave).  One sequence of 8160 steps x 960 channels x
-// 16 states, bf16, with a gate: 30 + 39 us in the two passes, the vector pipes busy for 88 and 94 % of them; its bytes would take
+// 16 states, bf16, with a gate: 31 + 42 us in the two passes, the vector pipes busy for 89 and 94 % of them; its bytes would take
 // 12.  4080 sequences of 12 steps x 64 channels: 16.6 us, bytes 10.7.
 // Where there are too few (sequence, 64 channels) pairs for the chip, the time axis is cut into chunks, a wave each, the waves
 // of a block being neighbours.  ENDS computes each chunk's last state from a zero start and the sum of its step sizes, and
-// composes them over the block (the decay over a chunk is exp(A sum delta)): every chunk's first state within its block, and
+// composes them over the block (the decay over a chunk is exp(A sum delta), see carried): every chunk's first state within its block, and
 // the block's last.  FROM composes the blocks in front of it, then runs its chunks from there.
 enum ScanMode { SCAN_WHOLE, SCAN_ENDS, SCAN_FROM };
 constexpr int SCAN_WAVES = 8;                           // waves of a block where the time axis is cut (16: two thirds slower at 1021 steps)
