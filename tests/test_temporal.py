@@ -618,14 +618,16 @@ def test_attend_one_token_rounds_once(dtype, longest):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
-def test_attend_one_token_with_values_that_are_not_finite(dtype, bad):
-    """A value that is not finite decides its own dim, for the heads that read it, and touches no other."""
+@pytest.mark.parametrize("longest", [100, 3000])
+def test_attend_one_token_with_values_that_are_not_finite(dtype, bad, longest):
+    """A value that is not finite decides its own dim, for the heads that read it, and touches no other - in a segment that a block
+    has whole, and in one that is put together from pieces."""
     from robustvideomatting_amd import temporal as M
-    dt, g, lengths = DT[dtype], _gen(17), [100, 20]
+    dt, g, lengths = DT[dtype], _gen(17), [longest, 20]
     cache, table, rows, lens = _attend_case(g, lengths, [1, 1], 4, 2, 64, 16, dt, 0.0)
     q = _rn(g, 2, 4, 64, dtype=dt)
     clean, bound = O.attend(q, *cache, rows, lengths, parts=2 if dt != torch.float32 else 1)
-    for at, dim in ((0, 0), (37, 5), (100, 63)):
+    for at, dim in ((0, 0), (37, 5), (longest, 63)):
         cell = cache[1][rows[0][at // 16], 1, at % 16]
         keep = cell[dim].item()
         cell[dim] = bad
