@@ -189,7 +189,9 @@ typedef struct rvm_append_args {
 int rvm_append_kv(int dtype, const rvm_append_args* args, void* hip_stream);
 
 /* out[m,h] = sum_j softmax_j(scale * q[m,h] . k_j) v_j over the positions j <= the row's own; query head h reads key head
- * h / (Hq / Hkv).  Append the rows' own keys first. */
+ * h / (Hq / Hkv).  Append the rows' own keys first.  scale: positive and finite in fp32, also times log2 e.  Rows of more than
+ * 32 streams (with offsets) are not cut along their keys: where a few of many have much longer memories, calls of up to 32
+ * streams are faster. */
 typedef struct rvm_attend_args {
     const void *q, *k_pages, *v_pages; void *out, *workspace;   /* [M,Hq,Dh] by strides; out dense */
     const int32_t *table, *lengths, *offsets;

@@ -333,6 +333,9 @@ def attend(q, cache, table, lengths, offsets=None, scale=None):
     own, ``lengths[s] + i`` (the rows' own keys are appended first, with the same arguments).  ``q`` [M, heads, dim]; query
     head h reads key head ``h // (heads / kv heads)``; ``scale`` defaults to ``dim ** -0.5``.  Returns [M, heads, dim].
 
+    ``scale`` must be positive and finite in fp32.  Rows of more than 32 streams (with ``offsets``) are not cut along their keys: where
+    a few of many streams have much longer memories, calls of up to 32 streams are faster.
+
     A row with a negative position, or behind the last stream's rows, gives 0.  Pages outside the pool are not followed:
     a row that would read one gives NaN."""
     try:
